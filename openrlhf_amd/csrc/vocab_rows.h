@@ -1,10 +1,14 @@
 // Shared pieces of the vocabulary-row kernels: element traits (bf16 / fp16 / fp32 as 16-byte
-// vectors), row geometry, statistic modes and the per-element gradient.
+// vectors), row geometry, statistic modes, the per-element gradient, and the streaming pass of one
+// 256-thread workgroup over a row with its softmax accumulators.
 #pragma once
 #include "common.h"
 
 #ifndef ORLHF_NT_LOAD
 #define ORLHF_NT_LOAD 1
+#endif
+#ifndef ORLHF_ROW_UNROLL
+#define ORLHF_ROW_UNROLL 8
 #endif
 #ifndef ORLHF_NT_STORE
 #define ORLHF_NT_STORE 1
@@ -184,5 +188,185 @@ struct GradFn {
     }
   }
 };
+
+// ---------------------------------------------------------------- streaming pass over a row
+// Visits every element of a row exactly once. f.vec(x, v) gets the kPerVec consecutive elements
+// of body vector v (element index head + v*kPerVec); f.one(x, e) gets element e. With STORE the
+// (modified) values are written to out_row at the same element positions in the same dtype.
+// All in-row offsets are 32-bit: the row base stays in scalar registers.
+template <int DT, bool STORE, typename F>
+__device__ __forceinline__ void traverse_row(const char* row, char* out_row, const RowGeom& g,
+                                             F& f) {
+  using E = Elt<DT>;
+  constexpr uint32_t U = ORLHF_ROW_UNROLL;
+  constexpr uint32_t EPV = E::kPerVec;
+  const uint32_t tid = threadIdx.x;
+  const char* body = row + g.head * E::kSize;
+  char* obody = STORE ? out_row + g.head * E::kSize : nullptr;
+
+  const uint32_t nbatch = g.nvec / (kBlock * U);
+  uint32_t v0 = tid;
+  for (uint32_t b = 0; b < nbatch; ++b, v0 += kBlock * U) {
+    u32x4 buf[U];
+#pragma unroll
+    for (uint32_t u = 0; u < U; ++u) buf[u] = load_vec(body + (v0 + u * kBlock) * 16u);
+#pragma unroll
+    for (uint32_t u = 0; u < U; ++u) {
+      float x[EPV];
+      E::unpack(buf[u], x);
+      f.vec(x, v0 + u * kBlock);
+      if (STORE) store_vec(obody + (v0 + u * kBlock) * 16u, E::pack(x));
+    }
+  }
+  if (v0 < g.nvec) {  // last, partial batch: same loads in flight, predicated per vector
+    u32x4 buf[U];
+#pragma unroll
+    for (uint32_t u = 0; u < U; ++u) {
+      const uint32_t v = v0 + u * kBlock;
+      if (v < g.nvec) buf[u] = load_vec(body + v * 16u);
+    }
+#pragma unroll
+    for (uint32_t u = 0; u < U; ++u) {
+      const uint32_t v = v0 + u * kBlock;
+      if (v < g.nvec) {
+        float x[EPV];
+        E::unpack(buf[u], x);
+        f.vec(x, v);
+        if (STORE) store_vec(obody + v * 16u, E::pack(x));
+      }
+    }
+  }
+  // scalar head + tail (at most 2*(kPerVec-1) elements unless scalar_only)
+  const uint32_t nscalar = g.head + g.tail;
+  for (uint32_t k = tid; k < nscalar; k += kBlock) {
+    const uint32_t e = k < g.head ? k : g.head + g.nvec * EPV + (k - g.head);
+    float x = E::load1(row + e * E::kSize);
+    f.one(x, e);
+    if (STORE) E::store1(out_row + e * E::kSize, x);
+  }
+}
+
+constexpr int kAcc = 4;  // independent accumulators per lane
+
+// Fast path: exponent = x*c - M with a wave-uniform reference M (no running maximum).
+template <int MODE>
+struct FastAcc {
+  float cT, negMT, c1, negM1;
+  float sT[kAcc], s1[kAcc], t1[kAcc];
+  __device__ __forceinline__ void init(float m_ref, float c_scaled, float c_plain) {
+    cT = c_scaled;
+    c1 = c_plain;
+    negMT = -(m_ref * c_scaled);
+    negM1 = -(m_ref * c_plain);
+#pragma unroll
+    for (int k = 0; k < kAcc; ++k) sT[k] = s1[k] = t1[k] = 0.0f;
+  }
+  __device__ __forceinline__ void elem(float x, int k) {
+    if (ModeTraits<MODE>::kScaledSet) sT[k] += fast_exp2(fmaf(x, cT, negMT));
+    if (ModeTraits<MODE>::kPlainSet) {
+      const float e = fast_exp2(fmaf(x, c1, negM1));
+      s1[k] += e;
+      t1[k] = fmaf(e, x, t1[k]);
+    }
+  }
+  template <int N>
+  __device__ __forceinline__ void vec(float (&x)[N], uint32_t) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) elem(x[j], j % kAcc);
+  }
+  __device__ __forceinline__ void one(float& x, uint32_t) { elem(x, 0); }
+  __device__ __forceinline__ void fold(float& st, float& s, float& t) const {
+    st = (sT[0] + sT[1]) + (sT[2] + sT[3]);
+    s = (s1[0] + s1[1]) + (s1[2] + s1[3]);
+    t = (t1[0] + t1[1]) + (t1[2] + t1[3]);
+  }
+};
+
+// Safe path: per-lane running maximum m (raw logit units), sums relative to it.
+template <int MODE>
+struct SafeAcc {
+  float cT, c1;
+  float m, sT, s1, t1;
+  __device__ __forceinline__ void init(float c_scaled, float c_plain) {
+    cT = c_scaled;
+    c1 = c_plain;
+    m = -INFINITY;
+    sT = s1 = t1 = 0.0f;
+  }
+  __device__ __forceinline__ void raise(float cm) {
+    if (cm > m) {  // also true for the first finite element (m == -inf)
+      if (m != -INFINITY) {
+        const float d = m - cm;  // < 0, or -inf when cm == +inf
+        if (ModeTraits<MODE>::kScaledSet) sT *= fast_exp2(d * cT);
+        if (ModeTraits<MODE>::kPlainSet) {
+          const float r = fast_exp2(d * c1);
+          s1 *= r;
+          t1 *= r;
+        }
+      }
+      m = cm;
+    }
+  }
+  __device__ __forceinline__ void elem(float x) {
+    if (m == -INFINITY) {
+      // only -inf (or NaN) seen so far: exp() contributes 0 to the sums, but the reference's
+      // softmax(x)*x is 0 * -inf = NaN for such an element (a NaN logit poisons everything).
+      if (ModeTraits<MODE>::kPlainSet) t1 = NAN;
+      if (x != x) sT = s1 = NAN;
+      return;
+    }
+    // x == m covers m == +inf (inf - inf would be NaN): such an element counts as exp(0),
+    // which makes logsumexp +inf and the entropy NaN, as in the reference
+    const float d = (x == m) ? 0.0f : x - m;
+    if (ModeTraits<MODE>::kScaledSet) sT += fast_exp2(d * cT);
+    if (ModeTraits<MODE>::kPlainSet) {
+      const float e = fast_exp2(d * c1);
+      s1 += e;
+      t1 = fmaf(e, x, t1);
+    }
+  }
+  template <int N>
+  __device__ __forceinline__ void vec(float (&x)[N], uint32_t) {
+    float cm = x[0];
+#pragma unroll
+    for (int j = 1; j < N; ++j) cm = fmaxf(cm, x[j]);
+    raise(cm);
+#pragma unroll
+    for (int j = 0; j < N; ++j) elem(x[j]);
+  }
+  __device__ __forceinline__ void one(float& x, uint32_t) {
+    raise(x);
+    elem(x);
+  }
+};
+
+// Workgroup-combined sums. Fast pass: exponents were x*c - M, MT / M1 hold M (log2 units).
+// Safe pass: exponents were (x - m)*c, MT and M1 both hold the row maximum m (logit units).
+struct RowSums {
+  float MT, sT, M1, s1, t1;
+};
+
+__device__ __forceinline__ bool sums_usable(float s) { return s > 0.0f && s < INFINITY; }
+
+// Zero-fills a row without reading it.
+template <int DT>
+__device__ __forceinline__ void zero_row(char* out_row, const RowGeom& g) {
+  using E = Elt<DT>;
+  const uint32_t tid = threadIdx.x;
+  char* obody = out_row + g.head * E::kSize;
+  const u32x4 z = {0u, 0u, 0u, 0u};
+  for (uint32_t v = tid; v < g.nvec; v += kBlock) store_vec(obody + v * 16u, z);
+  const uint32_t nscalar = g.head + g.tail;
+  for (uint32_t k = tid; k < nscalar; k += kBlock) {
+    const uint32_t e = k < g.head ? k : g.head + g.nvec * E::kPerVec + (k - g.head);
+    E::store1(out_row + e * E::kSize, 0.0f);
+  }
+}
+
+inline int grid_for_rows(int64_t n_rows) {
+  // one workgroup per row; cap the grid and stride over rows beyond it
+  const int64_t cap = 1 << 20;
+  return (int)(n_rows < cap ? n_rows : cap);
+}
 
 }  // namespace orlhf
