@@ -154,6 +154,39 @@ int orlhf_logprob_entropy_bwd(const void* logits, void* grad_logits, int dtype, 
                               const uint8_t* row_mask, orlhf_stream_t stream);
 
 /*
+ * Log-prob of a given token, entropy and the k most likely tokens of every vocabulary row:
+ *   logprob, entropy   what orlhf_logprob_entropy_fwd computes, same labels (logprob NULL: not
+ *                      wanted, labels may be NULL; entropy NULL: not wanted). Logits of -inf or of
+ *                      their type's lowest value have weight 0 in the entropy, and a row of nothing
+ *                      but the lowest value is a uniform distribution
+ *   top_ids            int64 [n_rows, k]: the ids of the k largest logits of the row, descending,
+ *                      equal logits by ascending id (-0 equals +0; a NaN ranks before everything)
+ *   top_logprob        float [n_rows, k]: logits[i, id] / temperature - lse(logits[i] / temperature)
+ *   row_stats          float [n_rows, 4] or NULL: what orlhf_top_logprobs_bwd needs of the softmax
+ * 1 <= k <= 128, k <= vocab. Rows with row_mask 0 are not read: ids -1, everything else 0. No
+ * reference counterpart: the alternatives extend openrlhf/models/utils.py:139-163,182-186.
+ */
+int orlhf_top_logprobs_fwd(const void* logits, int dtype, int64_t n_rows, int64_t vocab,
+                           int64_t row_stride, const int64_t* labels, double temperature, int64_t k,
+                           float* logprob, float* entropy, float* top_logprob, int64_t* top_ids,
+                           float* row_stats, const uint8_t* row_mask, orlhf_stream_t stream);
+
+/*
+ * Its backward, written in the logits dtype: orlhf_logprob_entropy_bwd's gradient plus
+ *   sum_k g_top[i,k] * (1[j==top_ids[i,k]] - softmax(logits/temperature)[i,j]) / temperature
+ * `grad_logits` may alias `logits` (same row stride). g_logprob, g_entropy float [n_rows] and
+ * g_top_logprob float [n_rows, k]: each may be NULL (zero), not all. The ids of a row have to be
+ * distinct, as the forward gives them; ids outside [0, vocab) get no one-hot term. Rows whose
+ * upstream gradients are all 0, or with row_mask 0, are written as zeros without being read.
+ */
+int orlhf_top_logprobs_bwd(const void* logits, void* grad_logits, int dtype, int64_t n_rows,
+                           int64_t vocab, int64_t row_stride, int64_t grad_row_stride,
+                           const int64_t* labels, double temperature, int64_t k,
+                           const int64_t* top_ids, const float* g_logprob, const float* g_entropy,
+                           const float* g_top_logprob, const float* row_stats,
+                           const uint8_t* row_mask, orlhf_stream_t stream);
+
+/*
  * Forward and backward in ONE pass for callers that know the upstream weights when the forward
  * runs, i.e. whose loss is sum_i w_logprob[i]*logprob[i] + w_entropy[i]*entropy[i] (SFT:
  * w_logprob = -mask/N, openrlhf/models/loss.py:104): computes logprob / entropy exactly as

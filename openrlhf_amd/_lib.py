@@ -24,6 +24,7 @@ PAIR_DPO_SIGMOID, PAIR_DPO_IPO, PAIR_LOGSIGMOID, PAIR_LOGEXP = 0, 1, 2, 3
 
 ABI_VERSION = 23
 UNPAD_TILE = 2048  # ORLHF_UNPAD_TILE
+LIST_MAX = 128  # longest list of tokens per vocabulary row (alternatives, a teacher's top tokens)
 
 
 class Norm(Structure):
@@ -82,6 +83,8 @@ SIGNATURES = {
     "orlhf_logprob_entropy_bwd": (c_int, [P, P, c_int, I64, I64, I64, I64, P, c_double, P, P, P, P, P]),
     "orlhf_logprob_entropy_fwd_bwd_max_vocab": (I64, [c_int]),
     "orlhf_logprob_entropy_fwd_bwd": (c_int, [P, P, c_int, I64, I64, I64, I64, P, c_double, P, P, P, P, P, P]),
+    "orlhf_top_logprobs_fwd": (c_int, [P, c_int, I64, I64, I64, P, c_double, I64, P, P, P, P, P, P, P]),
+    "orlhf_top_logprobs_bwd": (c_int, [P, P, c_int, I64, I64, I64, I64, P, c_double, I64, P, P, P, P, P, P, P]),
     "orlhf_lmhead_workspace_bytes": (I64, [I64, I64, I64, I64, c_int]),
     "orlhf_lmhead_logprob_entropy_fwd": (c_int, [P, P, c_int, I64, I64, I64, I64, I64, P, c_double, P, P, P, P, I64, I64,
                                                  P, I64, P]),

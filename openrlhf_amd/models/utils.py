@@ -10,7 +10,8 @@ Mirrors (paths relative to the OpenRLHF tree):
 plus ``logprobs_and_entropy_from_logits``, the one-pass form of what Actor.forward does with
 two calls (openrlhf/models/actor.py:269-285), and ``lm_head_logprobs_and_entropy``, the same from
 the last hidden states and the lm_head weight with the logits never stored
-(openrlhf/models/actor.py:263-285).
+(openrlhf/models/actor.py:263-285). ``top_logprobs_from_logits`` adds the k most likely tokens of
+every position to the one-pass form (no reference counterpart).
 
 Every function launches hand-written HIP kernels through the C ABI; tensors must be on the GPU.
 
@@ -211,6 +212,113 @@ def compute_entropy(logits: torch.Tensor, inplace_backward: bool = False) -> tor
     """logsumexp(x) - sum(softmax(x) * x) over the last dim (openrlhf/models/utils.py:182-186),
     fp32 result."""
     return _LogprobEntropy.apply(logits, None, 1.0, False, True, inplace_backward)[1]
+
+
+# ------------------------------------------------------------------ the k most likely tokens of a row
+def _mask_rows(row_mask, batch_shape):
+    """uint8 [n_rows] of a row mask of any dtype, or None."""
+    if row_mask is None:
+        return None
+    if row_mask.shape != batch_shape:
+        raise ValueError(f"row_mask shape {tuple(row_mask.shape)} != logits batch shape {tuple(batch_shape)}")
+    return (row_mask != 0).reshape(-1).to(torch.uint8).contiguous()
+
+
+def _f32_rows(t, shape, name):
+    """Contiguous fp32 [prod(shape)] of a per-row tensor, or None."""
+    if t is None:
+        return None
+    if t.shape != shape:
+        raise ValueError(f"{name} shape {tuple(t.shape)} != {tuple(shape)}")
+    return t.to(torch.float32).contiguous()
+
+
+class _TopLogprobs(torch.autograd.Function):
+    """logits -> (log-prob of label, entropy, log-probs of the k most likely tokens, their ids)."""
+
+    @staticmethod
+    def forward(ctx, logits, labels, k, temperature, want_entropy, inplace_backward, row_mask):
+        dev = require_gpu(logits, labels, row_mask)
+        code = _lib.dtype_code(logits)
+        batch_shape = logits.shape[:-1]
+        if labels is not None and labels.shape != batch_shape:
+            raise ValueError(f"labels shape {tuple(labels.shape)} != logits batch shape {tuple(batch_shape)}")
+        if not 1 <= k <= min(_lib.LIST_MAX, logits.shape[-1]):
+            raise ValueError(f"k={k} must lie in 1..{_lib.LIST_MAX} and not exceed the vocabulary ({logits.shape[-1]})")
+        rows, row_stride, aliases = _as_rows(logits.detach())
+        n_rows, vocab = rows.shape
+        lab = None if labels is None else labels.reshape(-1).to(torch.int64).contiguous()
+        rmask = _mask_rows(row_mask, batch_shape)
+        needs_grad = ctx.needs_input_grad[0]
+        opts = dict(device=dev, dtype=torch.float32)
+        logprob = torch.empty(n_rows, **opts) if lab is not None else None
+        entropy = torch.empty(n_rows, **opts) if want_entropy else None
+        top = torch.empty((n_rows, k), **opts)
+        ids = torch.empty((n_rows, k), device=dev, dtype=torch.int64)
+        stats = torch.empty((n_rows, 4), **opts) if needs_grad else None
+        with _lib.on_device(dev):
+            call("orlhf_top_logprobs_fwd", ptr(rows), code, n_rows, vocab, row_stride, ptr(lab), float(temperature), k,
+                 ptr(logprob), ptr(entropy), ptr(top), ptr(ids), ptr(stats), ptr(rmask), stream_of(dev))
+        ctx.temperature, ctx.k = float(temperature), k
+        ctx.inplace = bool(inplace_backward) and aliases
+        ctx.row_stride = row_stride
+        ctx.logits_shape = logits.shape
+        ctx.set_materialize_grads(False)
+        top_ids = ids.view(*batch_shape, k)
+        ctx.mark_non_differentiable(top_ids)
+        if needs_grad:
+            ctx.save_for_backward(rows, lab, ids, stats, rmask)
+        return (None if logprob is None else logprob.view(batch_shape),
+                None if entropy is None else entropy.view(batch_shape), top.view(*batch_shape, k), top_ids)
+
+    @staticmethod
+    def backward(ctx, g_logprob, g_entropy, g_top, _g_ids):
+        none = (None,) * 7
+        if g_logprob is None and g_entropy is None and g_top is None:
+            return none
+        rows, lab, ids, stats, rmask = ctx.saved_tensors
+        dev = rows.device
+        n_rows, vocab = rows.shape
+
+        def flat(g):
+            return None if g is None else g.to(torch.float32).contiguous()
+
+        glp, gent, gtop = flat(g_logprob), flat(g_entropy), flat(g_top)
+        if ctx.inplace:
+            grad_rows, grad_stride = rows, ctx.row_stride
+        else:
+            grad_rows, grad_stride = torch.empty((n_rows, vocab), device=dev, dtype=rows.dtype), vocab
+        with _lib.on_device(dev):
+            call("orlhf_top_logprobs_bwd", ptr(rows), ptr(grad_rows), _lib.dtype_code(rows), n_rows, vocab, ctx.row_stride,
+                 grad_stride, ptr(lab), ctx.temperature, ctx.k, ptr(ids), ptr(glp), ptr(gent), ptr(gtop), ptr(stats),
+                 ptr(rmask), stream_of(dev))
+        if grad_rows is rows:  # as in _LogprobEntropy: the saved logits are gone
+            torch.autograd.graph.increment_version(rows)
+        grad = grad_rows if grad_rows.shape == ctx.logits_shape else grad_rows.view(ctx.logits_shape)
+        return (grad,) + none[1:]
+
+
+def top_logprobs_from_logits(
+    logits: torch.Tensor,
+    labels: Optional[torch.Tensor],
+    k: int,
+    temperature: float = 1.0,
+    return_entropy: bool = True,
+    inplace_backward: bool = False,
+    row_mask: Optional[torch.Tensor] = None,
+) -> Tuple[Optional[torch.Tensor], Optional[torch.Tensor], torch.Tensor, torch.Tensor]:
+    """``logprobs_and_entropy_from_logits`` together with the ``k`` most likely tokens of every row:
+    ``(log_probs [...], entropy [...], top_log_probs [..., k], top_ids [..., k])``.
+
+    The alternatives are the k largest logits, descending, equal logits by ascending id (a NaN ranks
+    before everything); their log-probs, like the label's, are those of ``logits / temperature``, the
+    entropy is that of the unscaled logits. ``labels=None`` leaves the log-probs out (None is
+    returned), ``return_entropy=False`` the entropy. ``1 <= k <= 128``.
+
+    Differentiable in the three float outputs (the choice of the tokens is taken as given).
+    ``inplace_backward`` and ``row_mask`` as in ``logprobs_and_entropy_from_logits``; a position with
+    mask 0 gets ids -1 and zeros."""
+    return _TopLogprobs.apply(logits, labels, int(k), temperature, bool(return_entropy), inplace_backward, row_mask)
 
 
 # ------------------------------------------------------------------ lm-head + log-prob, logits not stored

@@ -339,3 +339,34 @@ def test_row_order_from_the_host_must_be_a_permutation():
             _order_arg(torch.tensor(bad), 4, cpu)
     with pytest.raises(ValueError, match="entries"):
         _order_arg(torch.tensor([0, 1, 2]), 4, cpu)
+
+
+def test_top_logprobs_entries_refuse_bad_arguments(lib):
+    import torch
+
+    from openrlhf_amd.models.utils import top_logprobs_from_logits
+
+    def err():
+        return lib.orlhf_last_error().decode()
+
+    fwd = lambda n=2, v=64, stride=64, t=1.0, k=4, x=8, dt=1, top=8: lib.orlhf_top_logprobs_fwd(  # noqa: E731
+        x, dt, n, v, stride, None, t, k, None, None, top, 8, None, None, None)
+    assert fwd(k=0) == -1 and "k=0" in err()
+    assert fwd(k=129, v=1000, stride=1000) == -1 and "k=129" in err()
+    assert fwd(k=65) == -1 and "exceed vocab" in err()
+    assert fwd(stride=63) == -1 and "row_stride" in err()
+    assert fwd(v=1 << 29, stride=1 << 29) == -1 and "too large" in err()
+    for t in (0.0, -1.0, float("nan"), float("inf")):
+        assert fwd(t=t) == -1 and "temperature" in err()
+    assert fwd(dt=5) == -1 and "dtype" in err()
+    assert fwd(x=9) == -1 and "aligned" in err()
+    assert fwd(top=None) == -1 and "NULL" in err()
+    assert fwd(n=0, x=None) == 0
+    bwd = lambda glp=None, gh=None, gtop=None, ids=None, gs=64: lib.orlhf_top_logprobs_bwd(  # noqa: E731
+        8, 8, 1, 2, 64, 64, gs, None, 1.0, 4, ids, glp, gh, gtop, 8, None, None)
+    assert bwd() == -1 and "every upstream" in err()
+    assert bwd(glp=8) == -1 and "labels" in err()
+    assert bwd(gtop=8) == -1 and "top_ids" in err()
+    assert bwd(gh=8, gs=63) == -1 and "grad_row_stride" in err()
+    with pytest.raises(RuntimeError, match="GPU only"):
+        top_logprobs_from_logits(torch.zeros(2, 8), None, 2)
