@@ -32,6 +32,24 @@ struct Candidates {
   int count;
 };
 
+// How many of the n candidates rank before each of this thread's (at threadIdx.x + i * kBlock).
+template <int MINE>
+__device__ __forceinline__ void rank_candidates(const Candidates& c, int n, uint64_t (&mine)[MINE], int (&rank)[MINE]) {
+#pragma unroll
+  for (int i = 0; i < MINE; ++i) {
+    const int at = (int)threadIdx.x + i * kBlock;
+    mine[i] = at < n ? c.key[at] : 0ull;
+    rank[i] = 0;
+  }
+  if ((int)(threadIdx.x & ~(kWave - 1u)) >= n) return;  // a wave without a candidate
+#pragma unroll 4
+  for (int j = 0; j < n; ++j) {
+    const uint64_t other = c.key[j];
+#pragma unroll
+    for (int i = 0; i < MINE; ++i) rank[i] += other > mine[i] ? 1 : 0;
+  }
+}
+
 // Keeps the k best candidates, sorted, and returns the k-th (0 while there are fewer). The whole
 // workgroup calls it with the candidates in place behind a barrier; another one ends it.
 __device__ __forceinline__ uint64_t keep_best(Candidates& c, int k) {
@@ -39,17 +57,7 @@ __device__ __forceinline__ uint64_t keep_best(Candidates& c, int k) {
   const int n = c.count;
   uint64_t mine[kMine];
   int rank[kMine];
-#pragma unroll
-  for (int i = 0; i < kMine; ++i) {
-    const int at = (int)threadIdx.x + i * kBlock;
-    mine[i] = at < n ? c.key[at] : 0ull;
-    rank[i] = 0;
-  }
-  for (int j = 0; j < n; ++j) {
-    const uint64_t other = c.key[j];
-#pragma unroll
-    for (int i = 0; i < kMine; ++i) rank[i] += other > mine[i] ? 1 : 0;
-  }
+  rank_candidates<kMine>(c, n, mine, rank);
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < kMine; ++i) {
@@ -114,6 +122,7 @@ struct TopArgs {
   float *logprob, *entropy, *top_logprob, *row_stats;  // logprob, entropy, row_stats may be NULL
   int64_t* top_ids;
   const uint8_t* row_mask;
+  int shift;  // of the selection's blocks
 };
 
 __device__ __forceinline__ void write_skipped_row(const TopArgs& a, int64_t row_i) {
@@ -305,11 +314,154 @@ __device__ __forceinline__ float logprob_of(float x, double temperature, const R
   return (float)(((double)x / temperature - r.base) - r.log_sum);
 }
 
+// ---------------------------------------------------------------- selection
+// The streaming pass leaves, beside the sums, the maximum of every BLOCK of a thread's elements in
+// LDS (a block: 4 vectors, or 4 << shift where a row has more than kMaxBlocks such blocks per
+// thread) and the maximum of all of them in a register: half an operation per element. The k-th
+// largest of the 256 thread maxima is a lower bound of the row's k-th largest logit that few more
+// than k elements pass (expected -256 ln(1 - k/256): 20 for k = 20, 177 for k = 128), so only the
+// blocks that reach it are read again, a few KiB per row, and their elements that reach it become
+// candidates. A row that has more of them than fit (many equal logits), or a NaN, goes through
+// collect_row instead.
+constexpr int kMaxBlocks = 32;
+constexpr uint32_t kBlockVecs = 4;  // vectors of one thread in a block (shift 0)
+
 template <int DT, int MODE>
-__global__ __launch_bounds__(kBlock) void top_logprobs_fwd_kernel(TopArgs a) {
+__device__ __forceinline__ float stream_row(const char* row, const RowGeom& g, FastAcc<MODE>& acc, float* block_max,
+                                            int shift) {
+  using E = Elt<DT>;
+  constexpr uint32_t U = ORLHF_ROW_UNROLL;
+  static_assert(U % kBlockVecs == 0, "a batch holds whole blocks");
+  const uint32_t tid = threadIdx.x;
+  const char* body = row + g.head * E::kSize;
+  float thread_max = -INFINITY;
+  auto take = [&](const u32x4& raw, float& bm, uint32_t v) {
+    float x[E::kPerVec];
+    E::unpack(raw, x);
+#pragma unroll
+    for (int j = 0; j < E::kPerVec; ++j) bm = fmaxf(bm, x[j]);
+    acc.vec(x, v);
+  };
+  auto note = [&](uint32_t part, float bm) {  // part: which group of kBlockVecs vectors of the thread
+    float* slot = block_max + (part >> shift) * kBlock + tid;
+    *slot = (part & ((1u << shift) - 1u)) == 0u ? bm : fmaxf(*slot, bm);
+    thread_max = fmaxf(thread_max, bm);
+  };
+  const uint32_t nbatch = g.nvec / (kBlock * U);
+  uint32_t v0 = tid, part = 0;
+  for (uint32_t b = 0; b < nbatch; ++b, v0 += kBlock * U) {
+    u32x4 buf[U];
+#pragma unroll
+    for (uint32_t u = 0; u < U; ++u) buf[u] = load_vec(body + (v0 + u * kBlock) * 16u);
+#pragma unroll
+    for (uint32_t h = 0; h < U; h += kBlockVecs) {
+      float bm = -INFINITY;
+#pragma unroll
+      for (uint32_t u = h; u < h + kBlockVecs; ++u) take(buf[u], bm, v0 + u * kBlock);
+      note(part++, bm);
+    }
+  }
+  if (nbatch * kBlock * U < g.nvec) {  // the last, partial batch
+    u32x4 buf[U];
+#pragma unroll
+    for (uint32_t u = 0; u < U; ++u)
+      if (v0 + u * kBlock < g.nvec) buf[u] = load_vec(body + (v0 + u * kBlock) * 16u);
+#pragma unroll
+    for (uint32_t h = 0; h < U; h += kBlockVecs) {
+      if ((nbatch * U + h) * kBlock < g.nvec) {
+        float bm = -INFINITY;
+#pragma unroll
+        for (uint32_t u = h; u < h + kBlockVecs; ++u)
+          if (v0 + u * kBlock < g.nvec) take(buf[u], bm, v0 + u * kBlock);
+        note(part++, bm);
+      }
+    }
+  }
+  const uint32_t nscalar = g.head + g.tail;
+  for (uint32_t k = tid; k < nscalar; k += kBlock) {
+    const uint32_t e = k < g.head ? k : g.head + g.nvec * E::kPerVec + (k - g.head);
+    float x = E::load1(row + e * E::kSize);
+    acc.one(x, e);
+  }
+  return thread_max;
+}
+
+// The largest value of 16 leading bits that at least k of the 256 maxima reach, as ordered bits: one
+// wave, four maxima per lane, one counting step per bit.
+__device__ __forceinline__ uint32_t kth_maximum(const float* thread_max, int k) {
+  const int lane = threadIdx.x & (kWave - 1);
+  const f32x4 m = *(const f32x4*)(thread_max + lane * 4);
+  uint32_t o[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) o[i] = ordered_bits(m[i]);
+  uint32_t found = 0;
+#pragma unroll
+  for (int bit = 31; bit >= 16; --bit) {
+    const uint32_t probe = found | (1u << bit);
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) n += __popcll(__ballot(o[i] >= probe));
+    if (n >= k) found = probe;
+  }
+  return found;
+}
+
+// The elements that reach `bar` in the blocks that do, into the candidates (their count may pass
+// kCap: then not all are there).
+template <int DT>
+__device__ __forceinline__ void collect_blocks(const char* row, const RowGeom& g, uint32_t first, const float* block_max,
+                                               int shift, float bar, float thread_max, Candidates& c) {
+  using E = Elt<DT>;
+  const uint32_t tid = threadIdx.x;
+  const char* body = row + g.head * E::kSize;
+  auto push = [&](float x, uint32_t id) {
+    if (x >= bar) {
+      const int at = atomicAdd(&c.count, 1);
+      if (at < kCap) c.key[at] = make_key(x, id);
+    }
+  };
+  if (thread_max >= bar) {
+    const uint32_t parts = (g.nvec + kBlockVecs * kBlock - 1) / (kBlockVecs * kBlock);
+    const uint32_t blocks = (parts + (1u << shift) - 1u) >> shift;
+    uint32_t wanted = 0;
+    for (uint32_t b = 0; b < blocks; ++b) wanted |= (block_max[b * kBlock + tid] >= bar ? 1u : 0u) << b;
+    while (wanted != 0u) {
+      const uint32_t b = (uint32_t)__builtin_ctz(wanted);
+      wanted &= wanted - 1u;
+      for (uint32_t part = b << shift; part < (b + 1u) << shift; ++part) {
+        u32x4 raw[kBlockVecs];
+        const uint32_t v0 = part * (kBlockVecs * kBlock) + tid;
+#pragma unroll
+        for (uint32_t u = 0; u < kBlockVecs; ++u)
+          if (v0 + u * kBlock < g.nvec) raw[u] = *(const u32x4*)(body + (v0 + u * kBlock) * 16u);
+#pragma unroll
+        for (uint32_t u = 0; u < kBlockVecs; ++u) {
+          const uint32_t v = v0 + u * kBlock;
+          if (v < g.nvec) {
+            float x[E::kPerVec];
+            E::unpack(raw[u], x);
+#pragma unroll
+            for (int j = 0; j < E::kPerVec; ++j) push(x[j], first + g.head + v * E::kPerVec + j);
+          }
+        }
+      }
+    }
+  }
+  const uint32_t nscalar = g.head + g.tail;
+  for (uint32_t k = tid; k < nscalar; k += kBlock) {
+    const uint32_t e = k < g.head ? k : g.head + g.nvec * E::kPerVec + (k - g.head);
+    push(E::load1(row + e * E::kSize), first + e);
+  }
+}
+
+template <int DT, int MODE>
+__global__ __launch_bounds__(kBlock, 4) void top_logprobs_fwd_kernel(TopArgs a) {
   using E = Elt<DT>;
   __shared__ float lds[kWavesPerBlock][8];
   __shared__ Candidates cand;
+  __shared__ alignas(16) float thread_maxima[kBlock];
+  __shared__ uint32_t bar_bits;
+  extern __shared__ float block_max[];
   const int tid = threadIdx.x;
   const float c_scaled = (float)(1.4426950408889634 / a.temperature);
   for (int64_t row_i = blockIdx.x; row_i < a.n_rows; row_i += gridDim.x) {
@@ -320,27 +472,53 @@ __global__ __launch_bounds__(kBlock) void top_logprobs_fwd_kernel(TopArgs a) {
     const char* row = a.logits + row_i * a.row_stride_bytes;
     const RowGeom g = row_geom<DT>(row, a.vocab, false);
     if (tid == 0) cand.count = 0;
+    // the label and its logit are asked for now and used by the row's last instructions
+    int64_t label = -1;
+    float x_label = 0.0f;
+    if (a.logprob != nullptr && tid == 0) {
+      label = a.labels[row_i];
+      if (label >= 0 && label < a.vocab) x_label = E::load1(row + label * E::kSize);
+    }
     FastAcc<MODE> acc;
     acc.init(wave_reference<DT>(row, g, (uint32_t)a.vocab), c_scaled, kLog2e);
-    traverse_row<DT, false>(row, nullptr, g, acc);
-    const RowSoftmax r = row_softmax<DT, MODE>(row, g, combine_fast<MODE>(acc, lds), c_scaled, a.temperature, lds);
-
-    collect_row<DT>(row, g, 0u, a.k, 0ull, cand);
-    keep_best(cand, a.k);
-    if (tid < a.k) {
-      const uint64_t key = cand.key[tid];
-      a.top_ids[row_i * a.k + tid] = (int64_t)key_id(key);
-      a.top_logprob[row_i * a.k + tid] = logprob_of(ordered_value((uint32_t)(key >> 32)), a.temperature, r);
+    const float thread_max = stream_row<DT, MODE>(row, g, acc, block_max, a.shift);
+    thread_maxima[tid] = thread_max;
+    const RowSums sums = combine_fast<MODE>(acc, lds);  // its barriers also publish the maxima
+    if (tid < kWave) {
+      const uint32_t bits = kth_maximum(thread_maxima, a.k);
+      if (tid == 0) bar_bits = bits;
+    }
+    const RowSoftmax mine = row_softmax<DT, MODE>(row, g, sums, c_scaled, a.temperature, lds);
+    __syncthreads();
+    const uint32_t bits = bar_bits;
+    const float bar = bits <= ordered_bits(-INFINITY) ? -INFINITY : ordered_value(bits);
+    collect_blocks<DT>(row, g, 0u, block_max, a.shift, bar, thread_max, cand);
+    __syncthreads();
+    int n = cand.count;
+    if (n > kCap || mine.nan) {
+      __syncthreads();
+      if (tid == 0) cand.count = 0;
+      collect_row<DT>(row, g, 0u, a.k, bits != 0u ? ((uint64_t)bits << 32) - 1u : 0ull, cand);
+      n = cand.count;
+    }
+    auto out = [&](uint64_t key, int at) {
+      a.top_ids[row_i * a.k + at] = (int64_t)key_id(key);
+      a.top_logprob[row_i * a.k + at] = logprob_of(ordered_value((uint32_t)(key >> 32)), a.temperature, mine);
+    };
+    if (n <= kBlock) {
+      uint64_t key[1];
+      int rank[1];
+      rank_candidates<1>(cand, n, key, rank);
+      if (tid < n && rank[0] < a.k) out(key[0], rank[0]);
+    } else {
+      keep_best(cand, a.k);
+      if (tid < a.k) out(cand.key[tid], tid);
     }
     if (tid == 0) {
-      if (a.logprob != nullptr) {
-        const int64_t label = a.labels[row_i];
-        const bool inside = label >= 0 && label < a.vocab;
-        a.logprob[row_i] = inside ? logprob_of(E::load1(row + label * E::kSize), a.temperature, r)
-                                  : (label == -100 ? 0.0f : NAN);
-      }
-      if (ModeTraits<MODE>::kPlainSet && a.entropy != nullptr) a.entropy[row_i] = (float)r.entropy;
-      if (a.row_stats != nullptr) *(f32x4*)(a.row_stats + row_i * 4) = f32x4{r.centre, r.l2_t, r.l2_1, r.ex};
+      if (a.logprob != nullptr)
+        a.logprob[row_i] = label >= 0 && label < a.vocab ? logprob_of(x_label, a.temperature, mine) : (label == -100 ? 0.0f : NAN);
+      if (ModeTraits<MODE>::kPlainSet && a.entropy != nullptr) a.entropy[row_i] = (float)mine.entropy;
+      if (a.row_stats != nullptr) *(f32x4*)(a.row_stats + row_i * 4) = f32x4{mine.centre, mine.l2_t, mine.l2_1, mine.ex};
     }
     __syncthreads();  // the candidates are read until here
   }
@@ -462,15 +640,19 @@ __global__ __launch_bounds__(kBlock) void top_logprobs_bwd_kernel(TopBwdArgs a) 
 }
 
 template <int DT>
-static int launch_top_fwd(const TopArgs& a, hipStream_t stream) {
+static int launch_top_fwd(TopArgs a, hipStream_t stream) {
   const bool t1 = a.temperature == 1.0;
+  const int64_t parts = (a.vocab / Elt<DT>::kPerVec + kBlockVecs * kBlock - 1) / (kBlockVecs * kBlock);
+  while ((parts + (1 << a.shift) - 1) >> a.shift > kMaxBlocks) ++a.shift;
+  const int64_t blocks = (parts + (1 << a.shift) - 1) >> a.shift;
+  const size_t lds = (size_t)(blocks > 0 ? blocks : 1) * kBlock * sizeof(float);
   const dim3 grid(grid_for_rows(a.n_rows)), block(kBlock);
   if (a.entropy == nullptr)
-    hipLaunchKernelGGL((top_logprobs_fwd_kernel<DT, kLpOnly>), grid, block, 0, stream, a);
+    hipLaunchKernelGGL((top_logprobs_fwd_kernel<DT, kLpOnly>), grid, block, lds, stream, a);
   else if (t1)
-    hipLaunchKernelGGL((top_logprobs_fwd_kernel<DT, kBothT1>), grid, block, 0, stream, a);
+    hipLaunchKernelGGL((top_logprobs_fwd_kernel<DT, kBothT1>), grid, block, lds, stream, a);
   else
-    hipLaunchKernelGGL((top_logprobs_fwd_kernel<DT, kBothT>), grid, block, 0, stream, a);
+    hipLaunchKernelGGL((top_logprobs_fwd_kernel<DT, kBothT>), grid, block, lds, stream, a);
   ORLHF_CHECK_LAUNCH("orlhf_top_logprobs_fwd");
   return ORLHF_OK;
 }
@@ -518,7 +700,7 @@ extern "C" int orlhf_top_logprobs_fwd(const void* logits, int dtype, int64_t n_r
                   "top_logprobs_fwd: logits not aligned to the element size");
   const int64_t esize = dtype == ORLHF_F32 ? 4 : 2;
   const TopArgs a = {(const char*)logits, n_rows, vocab, row_stride * esize, labels, temperature, (int)k, logprob,
-                     entropy, top_logprob, row_stats, top_ids, row_mask};
+                     entropy, top_logprob, row_stats, top_ids, row_mask, 0};
   hipStream_t s = (hipStream_t)stream;
   switch (dtype) {
     case ORLHF_F32: return launch_top_fwd<ORLHF_F32>(a, s);
