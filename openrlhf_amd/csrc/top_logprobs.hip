@@ -7,6 +7,8 @@
 // An element is one 64-bit key for the selection: the logit as an unsigned integer of the same
 // order in the high half, the complement of its id in the low half. Keys are unique, "greater"
 // means "ranked before", and a NaN (which has no order) ranks before everything.
+#include <type_traits>
+
 #include "vocab_rows.h"
 
 namespace orlhf {
@@ -28,8 +30,8 @@ __device__ __forceinline__ uint64_t make_key(float x, uint32_t id) {
 __device__ __forceinline__ uint32_t key_id(uint64_t key) { return 0xffffffffu - (uint32_t)key; }
 
 struct Candidates {
-  uint64_t key[kCap];
-  int count;
+  uint64_t* key;  // [kCap], LDS
+  int& count;
 };
 
 // How many of the n candidates rank before each of this thread's (at threadIdx.x + i * kBlock).
@@ -52,7 +54,7 @@ __device__ __forceinline__ void rank_candidates(const Candidates& c, int n, uint
 
 // Keeps the k best candidates, sorted, and returns the k-th (0 while there are fewer). The whole
 // workgroup calls it with the candidates in place behind a barrier; another one ends it.
-__device__ __forceinline__ uint64_t keep_best(Candidates& c, int k) {
+__device__ __forceinline__ uint64_t keep_best(const Candidates& c, int k) {
   constexpr int kMine = kCap / kBlock;
   const int n = c.count;
   uint64_t mine[kMine];
@@ -71,7 +73,7 @@ __device__ __forceinline__ uint64_t keep_best(Candidates& c, int k) {
 
 // Adds at most one key per thread, those above `least`; thins the candidates first when a whole
 // round might not fit. Called by the whole workgroup.
-__device__ __forceinline__ void push_round(Candidates& c, uint64_t key, int k, uint64_t& least) {
+__device__ __forceinline__ void push_round(const Candidates& c, uint64_t key, int k, uint64_t& least) {
   __syncthreads();
   const int n = c.count;
   __syncthreads();
@@ -83,11 +85,12 @@ __device__ __forceinline__ void push_round(Candidates& c, uint64_t key, int k, u
 // row (equal values, -inf, NaN), whatever the threshold `least` it starts from.
 template <int DT>
 __device__ __forceinline__ void collect_row(const char* row, const RowGeom& g, uint32_t first, int k, uint64_t least,
-                                            Candidates& c) {
+                                            const Candidates& c) {
   using E = Elt<DT>;
   constexpr int EPV = E::kPerVec;
   const uint32_t tid = threadIdx.x;
   const char* body = row + g.head * E::kSize;
+#pragma unroll 1
   for (uint32_t v0 = 0; v0 < g.nvec; v0 += kBlock) {
     const uint32_t v = v0 + tid;
     uint64_t key[EPV];
@@ -100,8 +103,13 @@ __device__ __forceinline__ void collect_row(const char* row, const RowGeom& g, u
       any = any || key[j] > least;
     }
     if (__syncthreads_or(any)) {
+#pragma unroll 1
+      for (int j = 0; j < EPV; ++j) {  // not unrolled: the candidates' thinning is a large piece of code
+        uint64_t mine = 0;
 #pragma unroll
-      for (int j = 0; j < EPV; ++j) push_round(c, key[j], k, least);
+        for (int i = 0; i < EPV; ++i) mine = i == j ? key[i] : mine;
+        push_round(c, mine, k, least);
+      }
     }
   }
   const uint32_t nscalar = g.head + g.tail;
@@ -112,6 +120,14 @@ __device__ __forceinline__ void collect_row(const char* row, const RowGeom& g, u
   }
   __syncthreads();
 }
+
+// One workgroup per row and no loop over rows in the kernels: a loop makes the compiler keep the
+// constants of the whole body (of the logarithms above all) in registers, 20 to 30 per lane.
+constexpr int64_t kGridX = 1 << 20;
+inline dim3 row_grid(int64_t n_rows) {
+  return dim3((unsigned)(n_rows < kGridX ? n_rows : kGridX), (unsigned)((n_rows + kGridX - 1) / kGridX));
+}
+__device__ __forceinline__ int64_t grid_row() { return (int64_t)blockIdx.y * kGridX + blockIdx.x; }
 
 struct TopArgs {
   const char* logits;
@@ -137,23 +153,6 @@ __device__ __forceinline__ void write_skipped_row(const TopArgs& a, int64_t row_
   }
 }
 
-// Wave reference of the fast pass: the maximum of the first vector (or scalar) of each lane.
-template <int DT>
-__device__ __forceinline__ float wave_reference(const char* row, const RowGeom& g, uint32_t len) {
-  using E = Elt<DT>;
-  float m = -INFINITY;
-  if (g.nvec > 0) {
-    const uint32_t v = threadIdx.x < g.nvec ? threadIdx.x : g.nvec - 1;
-    float x[E::kPerVec];
-    E::unpack(*(const u32x4*)(row + g.head * E::kSize + v * 16u), x);
-#pragma unroll
-    for (int j = 0; j < E::kPerVec; ++j) m = fmaxf(m, x[j]);
-  } else {
-    m = E::load1(row + (threadIdx.x < len ? threadIdx.x : len - 1) * E::kSize);
-  }
-  return wave_max(m);
-}
-
 // The softmax of a row as what its outputs and its backward need: base + log_sum is the
 // log-sum-exp of x / T (kept apart: base may be so large that the sum would be lost in it), `centre`
 // a logit near base * T that every later difference starts from, entropy and E[x] - centre those of
@@ -161,7 +160,6 @@ __device__ __forceinline__ float wave_reference(const char* row, const RowGeom& 
 struct RowSoftmax {
   double base, log_sum, entropy;
   float centre, l2_t, l2_1, ex;  // the backward's statistics: softmax(x / T) = 2^((x - centre) cT - l2_t)
-  bool nan;
 };
 
 // Fast pass: per wave sums against its reference, folded over the workgroup.
@@ -238,71 +236,99 @@ struct ExactAcc {
   }
 };
 
-// All threads of the workgroup get the same result. T = 1 (and entropy-free) modes keep one set.
+// The sums of a row in the form that finish_row takes: of 2^((x - ref) c), with the reference in log2
+// units after the fast pass and as a logit after the exact one.
+struct RowTotals {
+  float ref_t, ref_1;
+  double sT, s1, t1;  // t1: sum of e x (fast) or of e (x - ref) (exact)
+  bool fast, nan;
+};
+
+template <int MODE>
+__device__ __forceinline__ bool fast_usable(const RowSums& s) {
+  using MT = ModeTraits<MODE>;
+  bool ok = true;
+  if (MT::kScaledSet) ok = ok && sums_usable(s.sT) && fabsf(s.MT) < kFarReference;
+  if (MT::kPlainSet) ok = ok && sums_usable(s.s1) && fabsf(s.t1) < INFINITY && fabsf(s.M1) < kFarReference;
+  return ok;
+}
+
+// One vector per step: what only rare rows run must not cost the others their registers.
+template <int DT, typename F>
+__device__ __forceinline__ void walk_row(const char* row, const RowGeom& g, F& f) {
+  using E = Elt<DT>;
+  const uint32_t tid = threadIdx.x;
+  const char* body = row + g.head * E::kSize;
+#pragma unroll 1
+  for (uint32_t v = tid; v < g.nvec; v += kBlock) {
+    float x[E::kPerVec];
+    E::unpack(*(const u32x4*)(body + v * 16u), x);
+    f.vec(x, v);
+  }
+  if (tid < g.head + g.tail) {
+    const uint32_t e = tid < g.head ? tid : g.nvec * E::kPerVec + tid;
+    float x = E::load1(row + e * E::kSize);
+    f.one(x, e);
+  }
+}
+
 template <int DT, int MODE>
-__device__ __forceinline__ RowSoftmax row_softmax(const char* row, const RowGeom& g, RowSums sums, float c_scaled,
-                                                  double temperature, float (*lds)[8]) {
+__device__ __forceinline__ RowTotals exact_totals(const char* row, const RowGeom& g, float c_scaled, float (*lds)[8]) {
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+  MaxAcc top{-INFINITY, false};
+  walk_row<DT>(row, g, top);
+  const float m_w = wave_max(top.m);
+  const bool nan_w = __ballot(top.nan) != 0ull;
+  if (lane == 0) {
+    lds[wave][0] = m_w;
+    lds[wave][1] = nan_w ? 1.0f : 0.0f;
+  }
+  __syncthreads();
+  float m = lds[0][0], nans = lds[0][1];
+#pragma unroll
+  for (int w = 1; w < kWavesPerBlock; ++w) {
+    m = fmaxf(m, lds[w][0]);
+    nans += lds[w][1];
+  }
+  __syncthreads();
+  ExactAcc<MODE> acc{m, c_scaled, kLog2e, 0.0f, 0.0f, 0.0f};
+  walk_row<DT>(row, g, acc);
+  const float st = wave_sum(acc.sT), s = wave_sum(acc.s1), t = wave_sum(acc.t1);
+  if (lane == 0) {
+    lds[wave][0] = st;
+    lds[wave][1] = s;
+    lds[wave][2] = t;
+  }
+  __syncthreads();
+  RowTotals r = {m, m, 0.0, 0.0, 0.0, false, nans != 0.0f};
+#pragma unroll
+  for (int w = 0; w < kWavesPerBlock; ++w) {
+    r.sT += (double)lds[w][0];
+    r.s1 += (double)lds[w][1];
+    r.t1 += (double)lds[w][2];
+  }
+  __syncthreads();
+  if (r.nan || m == -INFINITY) r.sT = r.s1 = NAN;
+  if (m == INFINITY) r.t1 = NAN;
+  return r;
+}
+
+template <int MODE>
+__device__ __forceinline__ RowSoftmax finish_row(const RowTotals& t, double temperature) {
   using MT = ModeTraits<MODE>;
   RowSoftmax r;
-  bool ok = true;
-  if (MT::kScaledSet) ok = ok && sums_usable(sums.sT) && fabsf(sums.MT) < kFarReference;
-  if (MT::kPlainSet) ok = ok && sums_usable(sums.s1) && fabsf(sums.t1) < INFINITY && fabsf(sums.M1) < kFarReference;
-  r.nan = false;
-  double base_1, log_1, ex;  // of the unscaled logits; ex = E[x] - base_1
-  if (ok) {
-    r.base = (double)(MT::kScaledSet ? sums.MT : sums.M1) * kLn2d;
-    r.log_sum = log((double)(MT::kScaledSet ? sums.sT : sums.s1));
-    base_1 = (double)sums.M1 * kLn2d;
-    log_1 = MT::kPlainSet ? log((double)sums.s1) : 0.0;
-    ex = MT::kPlainSet ? (double)sums.t1 / (double)sums.s1 - base_1 : 0.0;
-  } else {
-    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-    MaxAcc top{-INFINITY, false};
-    traverse_row<DT, false>(row, nullptr, g, top);
-    const float m_w = wave_max(top.m);
-    const bool nan_w = __ballot(top.nan) != 0ull;
-    if (lane == 0) {
-      lds[wave][0] = m_w;
-      lds[wave][1] = nan_w ? 1.0f : 0.0f;
-    }
-    __syncthreads();
-    float m = lds[0][0], nans = lds[0][1];
-#pragma unroll
-    for (int w = 1; w < kWavesPerBlock; ++w) {
-      m = fmaxf(m, lds[w][0]);
-      nans += lds[w][1];
-    }
-    r.nan = nans != 0.0f;
-    __syncthreads();
-    ExactAcc<MODE> acc{m, c_scaled, kLog2e, 0.0f, 0.0f, 0.0f};
-    traverse_row<DT, false>(row, nullptr, g, acc);
-    const float st = wave_sum(acc.sT), s = wave_sum(acc.s1), t = wave_sum(acc.t1);
-    if (lane == 0) {
-      lds[wave][0] = st;
-      lds[wave][1] = s;
-      lds[wave][2] = t;
-    }
-    __syncthreads();
-    double sT = 0.0, s1 = 0.0, t1 = 0.0;
-#pragma unroll
-    for (int w = 0; w < kWavesPerBlock; ++w) {
-      sT += (double)lds[w][0];
-      s1 += (double)lds[w][1];
-      t1 += (double)lds[w][2];
-    }
-    __syncthreads();
-    if (r.nan || m == -INFINITY) sT = s1 = NAN;
-    if (m == INFINITY) t1 = NAN;
-    base_1 = (double)m;
-    r.base = (double)m / temperature;
-    r.log_sum = log(MT::kScaledSet ? sT : s1);
-    log_1 = log(s1);
-    ex = t1 / s1;
+  const double scale = MT::kScaledSet ? temperature : 1.0;  // one set serves both where T = 1
+  const double base_1 = t.fast ? (double)t.ref_1 * kLn2d : (double)t.ref_1;
+  double log_1 = 0.0, ex = 0.0;  // of the unscaled logits; ex = E[x] - base_1
+  if (MT::kPlainSet) {
+    log_1 = log(t.s1);
+    ex = t.t1 / t.s1 - (t.fast ? base_1 : 0.0);
   }
-  const double at = r.base * (MT::kScaledSet ? temperature : 1.0);
+  r.base = MT::kScaledSet ? (t.fast ? (double)t.ref_t * kLn2d : (double)t.ref_t / temperature) : base_1;
+  r.log_sum = MT::kScaledSet ? log(t.sT) : log_1;
+  const double at = r.base * scale;
   r.centre = (float)at;
-  const double shift = at - (double)r.centre;
-  r.l2_t = (float)((r.log_sum + shift / (MT::kScaledSet ? temperature : 1.0)) * 1.4426950408889634);
+  r.l2_t = (float)((r.log_sum + (at - (double)r.centre) / scale) * 1.4426950408889634);
   r.entropy = log_1 - ex;
   const double rest = base_1 - (double)r.centre;
   r.l2_1 = MT::kPlainSet ? (float)((log_1 + rest) * 1.4426950408889634) : 0.0f;
@@ -315,73 +341,102 @@ __device__ __forceinline__ float logprob_of(float x, double temperature, const R
 }
 
 // ---------------------------------------------------------------- selection
-// The streaming pass leaves, beside the sums, the maximum of every BLOCK of a thread's elements in
-// LDS (a block: 4 vectors, or 4 << shift where a row has more than kMaxBlocks such blocks per
-// thread) and the maximum of all of them in a register: half an operation per element. The k-th
-// largest of the 256 thread maxima is a lower bound of the row's k-th largest logit that few more
-// than k elements pass (expected -256 ln(1 - k/256): 20 for k = 20, 177 for k = 128), so only the
-// blocks that reach it are read again, a few KiB per row, and their elements that reach it become
-// candidates. A row that has more of them than fit (many equal logits), or a NaN, goes through
-// collect_row instead.
+// The streaming pass leaves, beside the sums, the maximum of every BLOCK of the row in LDS and the
+// maximum of all blocks of a thread in a register. A block is 64 consecutive bytes, the vectors that
+// four neighbouring lanes load with one instruction (64 << shift bytes in pieces where a row has more
+// than kMaxBlocks of them per thread); the four lanes exchange their maxima so that each keeps one of
+// the four blocks of a step: 0.8 operations per element in all. The k-th largest of the 256 thread
+// maxima is a lower bound of the row's k-th largest logit that few more than k elements pass
+// (expected -256 ln(1 - k/256): 20 for k = 20, 177 for k = 128), so only the blocks that reach it are
+// read again, about 64 k bytes per row, and their elements that reach it become candidates. (Blocks of
+// one lane's four vectors need no exchange but lie 4 KiB apart, and reading them again fetched an
+// eighth of the row: 221 against 197 us at 4096 x 151936 bf16, k = 64.) A row that has more candidates
+// than fit (many equal logits), or a NaN, goes through collect_row instead.
 constexpr int kMaxBlocks = 32;
-constexpr uint32_t kBlockVecs = 4;  // vectors of one thread in a block (shift 0)
+constexpr uint32_t kBlockVecs = 4;  // vectors in a block, and a thread's loads per step
 
+// Lane j of four gets the maximum over the four lanes of m[j].
+__device__ __forceinline__ float quad_maxima(const float (&m)[4]) {
+  const bool odd = (threadIdx.x & 1u) != 0u, high = (threadIdx.x & 2u) != 0u;
+  auto with_neighbour = [](float keep, float give, auto ctrl) {
+    constexpr int kCtrl = decltype(ctrl)::value;
+    return fmaxf(keep, as_float((uint32_t)__builtin_amdgcn_mov_dpp((int)as_uint(give), kCtrl, 0xf, 0xf, true)));
+  };
+  constexpr std::integral_constant<int, 0xB1> kSwap1{};  // quad_perm [1, 0, 3, 2]
+  constexpr std::integral_constant<int, 0x4E> kSwap2{};  // quad_perm [2, 3, 0, 1]
+  const float lo = with_neighbour(odd ? m[1] : m[0], odd ? m[0] : m[1], kSwap1);
+  const float hi = with_neighbour(odd ? m[3] : m[2], odd ? m[2] : m[3], kSwap1);
+  return with_neighbour(high ? hi : lo, high ? lo : hi, kSwap2);
+}
+
+// The loads of the next block are in flight while one is worked on: two blocks of registers, 16 KiB
+// asked for ahead by each workgroup at any time. The wave's exponent reference is the maximum of its
+// lanes' first blocks.
 template <int DT, int MODE>
-__device__ __forceinline__ float stream_row(const char* row, const RowGeom& g, FastAcc<MODE>& acc, float* block_max,
-                                            int shift) {
+__device__ __forceinline__ float stream_row(const char* row, const RowGeom& g, float c_scaled, FastAcc<MODE>& acc,
+                                            float* block_max, int shift) {
   using E = Elt<DT>;
-  constexpr uint32_t U = ORLHF_ROW_UNROLL;
-  static_assert(U % kBlockVecs == 0, "a batch holds whole blocks");
+  constexpr int EPV = E::kPerVec;
+  constexpr uint32_t kStep = kBlockVecs * kBlock;
   const uint32_t tid = threadIdx.x;
   const char* body = row + g.head * E::kSize;
   float thread_max = -INFINITY;
-  auto take = [&](const u32x4& raw, float& bm, uint32_t v) {
-    float x[E::kPerVec];
-    E::unpack(raw, x);
+  const uint32_t parts = (g.nvec + kStep - 1) / kStep;
+  auto load = [&](u32x4 (&raw)[kBlockVecs], uint32_t part) {  // past the end: the last vector again, not used
 #pragma unroll
-    for (int j = 0; j < E::kPerVec; ++j) bm = fmaxf(bm, x[j]);
-    acc.vec(x, v);
+    for (uint32_t u = 0; u < kBlockVecs; ++u) {
+      const uint32_t v = part * kStep + u * kBlock + tid;
+      raw[u] = load_vec(body + (v < g.nvec ? v : g.nvec - 1) * 16u);
+    }
   };
-  auto note = [&](uint32_t part, float bm) {  // part: which group of kBlockVecs vectors of the thread
+  auto consume = [&](const u32x4 (&raw)[kBlockVecs], uint32_t part) {
+    float m[kBlockVecs] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+    const uint32_t v0 = part * kStep + tid;
+    auto take = [&](uint32_t u) {
+      float x[EPV];
+      E::unpack(raw[u], x);
+#pragma unroll
+      for (int j = 0; j < EPV; ++j) m[u] = fmaxf(m[u], x[j]);
+      acc.vec(x, 0);
+    };
+    if ((part + 1) * kStep <= g.nvec) {
+#pragma unroll
+      for (uint32_t u = 0; u < kBlockVecs; ++u) take(u);
+    } else {
+#pragma unroll
+      for (uint32_t u = 0; u < kBlockVecs; ++u)
+        if (v0 + u * kBlock < g.nvec) take(u);
+    }
+    const float bm = quad_maxima(m);
     float* slot = block_max + (part >> shift) * kBlock + tid;
     *slot = (part & ((1u << shift) - 1u)) == 0u ? bm : fmaxf(*slot, bm);
     thread_max = fmaxf(thread_max, bm);
   };
-  const uint32_t nbatch = g.nvec / (kBlock * U);
-  uint32_t v0 = tid, part = 0;
-  for (uint32_t b = 0; b < nbatch; ++b, v0 += kBlock * U) {
-    u32x4 buf[U];
-#pragma unroll
-    for (uint32_t u = 0; u < U; ++u) buf[u] = load_vec(body + (v0 + u * kBlock) * 16u);
-#pragma unroll
-    for (uint32_t h = 0; h < U; h += kBlockVecs) {
-      float bm = -INFINITY;
-#pragma unroll
-      for (uint32_t u = h; u < h + kBlockVecs; ++u) take(buf[u], bm, v0 + u * kBlock);
-      note(part++, bm);
-    }
-  }
-  if (nbatch * kBlock * U < g.nvec) {  // the last, partial batch
-    u32x4 buf[U];
-#pragma unroll
-    for (uint32_t u = 0; u < U; ++u)
-      if (v0 + u * kBlock < g.nvec) buf[u] = load_vec(body + (v0 + u * kBlock) * 16u);
-#pragma unroll
-    for (uint32_t h = 0; h < U; h += kBlockVecs) {
-      if ((nbatch * U + h) * kBlock < g.nvec) {
-        float bm = -INFINITY;
-#pragma unroll
-        for (uint32_t u = h; u < h + kBlockVecs; ++u)
-          if (v0 + u * kBlock < g.nvec) take(buf[u], bm, v0 + u * kBlock);
-        note(part++, bm);
-      }
-    }
-  }
+  u32x4 ping[kBlockVecs], pong[kBlockVecs];
+  if (parts > 0) load(ping, 0);
+  // head and tail of a row off the 16-byte grid: at most one element per thread
   const uint32_t nscalar = g.head + g.tail;
-  for (uint32_t k = tid; k < nscalar; k += kBlock) {
-    const uint32_t e = k < g.head ? k : g.head + g.nvec * E::kPerVec + (k - g.head);
-    float x = E::load1(row + e * E::kSize);
-    acc.one(x, e);
+  float xs = -INFINITY;
+  if (tid < nscalar) xs = E::load1(row + (tid < g.head ? tid : g.nvec * EPV + tid) * E::kSize);
+  float m_ref = xs;
+  if (parts > 0) {
+#pragma unroll
+    for (uint32_t u = 0; u < kBlockVecs; ++u) {
+      float x[EPV];
+      E::unpack(ping[u], x);
+#pragma unroll
+      for (int j = 0; j < EPV; ++j) m_ref = fmaxf(m_ref, x[j]);
+    }
+  }
+  acc.init(wave_max(m_ref), c_scaled, kLog2e);
+  if (tid < nscalar) acc.one(xs, 0);
+  for (uint32_t part = 0; part < parts;) {
+    if (part + 1 < parts) load(pong, part + 1);
+    consume(ping, part);
+    if (++part >= parts) break;
+    if (part + 1 < parts) load(ping, part + 1);
+    consume(pong, part);
+    ++part;
   }
   return thread_max;
 }
@@ -406,121 +461,145 @@ __device__ __forceinline__ uint32_t kth_maximum(const float* thread_max, int k) 
   return found;
 }
 
-// The elements that reach `bar` in the blocks that do, into the candidates (their count may pass
-// kCap: then not all are there).
+// The elements that reach `bar` in the blocks that do, into the candidates. The blocks are listed
+// first, so that their vectors spread over the whole workgroup and all are asked for at once (each
+// thread reading its own blocks one after the other costs a memory latency per block: 260 against
+// 238 us at 4096 x 151936 bf16, k = 64). Counts beyond kListed or kCap mean that not everything is there.
+constexpr int kListed = 1024;
+struct BlockList {
+  uint16_t block[kListed];  // block number * 256 + thread
+  int count;
+};
+static_assert(kMaxBlocks * kBlock <= 65536, "a listed block fits 16 bits");
+
 template <int DT>
 __device__ __forceinline__ void collect_blocks(const char* row, const RowGeom& g, uint32_t first, const float* block_max,
-                                               int shift, float bar, float thread_max, Candidates& c) {
+                                               int shift, float bar, float thread_max, BlockList& list, const Candidates& c) {
   using E = Elt<DT>;
+  constexpr int EPV = E::kPerVec;
+  constexpr uint32_t kStep = kBlockVecs * kBlock;
   const uint32_t tid = threadIdx.x;
   const char* body = row + g.head * E::kSize;
-  auto push = [&](float x, uint32_t id) {
-    if (x >= bar) {
-      const int at = atomicAdd(&c.count, 1);
-      if (at < kCap) c.key[at] = make_key(x, id);
-    }
-  };
   if (thread_max >= bar) {
-    const uint32_t parts = (g.nvec + kBlockVecs * kBlock - 1) / (kBlockVecs * kBlock);
+    const uint32_t parts = (g.nvec + kStep - 1) / kStep;
     const uint32_t blocks = (parts + (1u << shift) - 1u) >> shift;
-    uint32_t wanted = 0;
-    for (uint32_t b = 0; b < blocks; ++b) wanted |= (block_max[b * kBlock + tid] >= bar ? 1u : 0u) << b;
-    while (wanted != 0u) {
-      const uint32_t b = (uint32_t)__builtin_ctz(wanted);
-      wanted &= wanted - 1u;
-      for (uint32_t part = b << shift; part < (b + 1u) << shift; ++part) {
-        u32x4 raw[kBlockVecs];
-        const uint32_t v0 = part * (kBlockVecs * kBlock) + tid;
+    for (uint32_t b = 0; b < blocks; ++b) {
+      if (block_max[b * kBlock + tid] >= bar) {
+        const int at = atomicAdd(&list.count, 1);
+        if (at < kListed) list.block[at] = (uint16_t)(b * kBlock + tid);
+      }
+    }
+  }
+  auto push = [&](float x, uint32_t id) {
+    const int at = atomicAdd(&c.count, 1);
+    if (at < kCap) c.key[at] = make_key(x, id);
+  };
+  __syncthreads();  // from here on the candidates take the place of the block maxima
+  const int listed = list.count;
+  const uint32_t nscalar = g.head + g.tail;
+  if (tid < nscalar) {
+    const uint32_t e = tid < g.head ? tid : g.nvec * EPV + tid;
+    const float x = E::load1(row + e * E::kSize);
+    if (x >= bar) push(x, first + e);
+  }
+  const uint32_t per_shift = 2u + (uint32_t)shift;  // log2 of the vectors in a block
+  static_assert(kBlockVecs == 4, "per_shift");
+  if (listed <= kListed) {
+    for (uint32_t i = tid; i < (uint32_t)listed << per_shift; i += kBlock) {
+      const uint32_t blk = list.block[i >> per_shift];
+      const uint32_t t = blk % kBlock, in = i & ((1u << per_shift) - 1u);
+      const uint32_t v = (((blk / kBlock) << shift) + in / kBlockVecs) * kStep + t % 4u * kBlock + (t & ~3u) + in % kBlockVecs;
+      if (v < g.nvec) {
+        float x[EPV];
+        E::unpack(*(const u32x4*)(body + v * 16u), x);
+        float m = x[0];
 #pragma unroll
-        for (uint32_t u = 0; u < kBlockVecs; ++u)
-          if (v0 + u * kBlock < g.nvec) raw[u] = *(const u32x4*)(body + (v0 + u * kBlock) * 16u);
+        for (int j = 1; j < EPV; ++j) m = fmaxf(m, x[j]);
+        if (m >= bar) {
 #pragma unroll
-        for (uint32_t u = 0; u < kBlockVecs; ++u) {
-          const uint32_t v = v0 + u * kBlock;
-          if (v < g.nvec) {
-            float x[E::kPerVec];
-            E::unpack(raw[u], x);
-#pragma unroll
-            for (int j = 0; j < E::kPerVec; ++j) push(x[j], first + g.head + v * E::kPerVec + j);
-          }
+          for (int j = 0; j < EPV; ++j)
+            if (x[j] >= bar) push(x[j], first + g.head + v * EPV + j);
         }
       }
     }
   }
-  const uint32_t nscalar = g.head + g.tail;
-  for (uint32_t k = tid; k < nscalar; k += kBlock) {
-    const uint32_t e = k < g.head ? k : g.head + g.nvec * E::kPerVec + (k - g.head);
-    push(E::load1(row + e * E::kSize), first + e);
-  }
 }
 
 template <int DT, int MODE>
-__global__ __launch_bounds__(kBlock, 4) void top_logprobs_fwd_kernel(TopArgs a) {
+__global__ __launch_bounds__(kBlock) void top_logprobs_fwd_kernel(TopArgs a) {
   using E = Elt<DT>;
   __shared__ float lds[kWavesPerBlock][8];
-  __shared__ Candidates cand;
+  __shared__ int n_cand;
+  __shared__ BlockList list;
   __shared__ alignas(16) float thread_maxima[kBlock];
   __shared__ uint32_t bar_bits;
-  extern __shared__ float block_max[];
+  __shared__ RowSoftmax softmax;
+  extern __shared__ uint64_t shared[];  // block maxima while the row streams by, candidates afterwards
+  float* const block_max = (float*)shared;
+  const Candidates cand = {shared, n_cand};
   const int tid = threadIdx.x;
   const float c_scaled = (float)(1.4426950408889634 / a.temperature);
-  for (int64_t row_i = blockIdx.x; row_i < a.n_rows; row_i += gridDim.x) {
-    if (a.row_mask != nullptr && a.row_mask[row_i] == 0) {
-      write_skipped_row(a, row_i);
-      continue;
-    }
-    const char* row = a.logits + row_i * a.row_stride_bytes;
-    const RowGeom g = row_geom<DT>(row, a.vocab, false);
+  const int64_t row_i = grid_row();
+  if (row_i >= a.n_rows) return;
+  if (a.row_mask != nullptr && a.row_mask[row_i] == 0) {
+    write_skipped_row(a, row_i);
+    return;
+  }
+  const char* row = a.logits + row_i * a.row_stride_bytes;
+  const RowGeom g = row_geom<DT>(row, a.vocab, false);
+  if (tid == 0) n_cand = list.count = 0;
+  // the label and its logit are asked for now and used by the row's last instructions
+  int64_t label = -1;
+  float x_label = 0.0f;
+  if (a.logprob != nullptr && tid == 0) {
+    label = a.labels[row_i];
+    if (label >= 0 && label < a.vocab) x_label = E::load1(row + label * E::kSize);
+  }
+  FastAcc<MODE> acc;
+  const float thread_max = stream_row<DT, MODE>(row, g, c_scaled, acc, block_max, a.shift);
+  thread_maxima[tid] = thread_max;
+  const RowSums sums = combine_fast<MODE>(acc, lds);  // its barriers also publish the maxima
+  const bool fast = fast_usable<MODE>(sums);
+  RowTotals totals = {sums.MT, sums.M1, sums.sT, sums.s1, sums.t1, true, false};
+  if (!fast) totals = exact_totals<DT, MODE>(row, g, c_scaled, lds);
+  const bool nan = totals.nan;
+  if (tid < kWave) {  // one wave finds the bar, another takes the logarithms
+    const uint32_t bits = kth_maximum(thread_maxima, a.k);
+    if (tid == 0) bar_bits = bits;
+  } else if (tid < 2 * kWave) {
+    const RowSoftmax r = finish_row<MODE>(totals, a.temperature);
+    if (tid == kWave) softmax = r;
+  }
+  __syncthreads();
+  const uint32_t bits = bar_bits;
+  const float bar = bits <= ordered_bits(-INFINITY) ? -INFINITY : ordered_value(bits);
+  collect_blocks<DT>(row, g, 0u, block_max, a.shift, bar, thread_max, list, cand);
+  __syncthreads();
+  int n = cand.count;
+  if (n > kCap || list.count > kListed || nan) {
+    __syncthreads();
     if (tid == 0) cand.count = 0;
-    // the label and its logit are asked for now and used by the row's last instructions
-    int64_t label = -1;
-    float x_label = 0.0f;
-    if (a.logprob != nullptr && tid == 0) {
-      label = a.labels[row_i];
-      if (label >= 0 && label < a.vocab) x_label = E::load1(row + label * E::kSize);
-    }
-    FastAcc<MODE> acc;
-    acc.init(wave_reference<DT>(row, g, (uint32_t)a.vocab), c_scaled, kLog2e);
-    const float thread_max = stream_row<DT, MODE>(row, g, acc, block_max, a.shift);
-    thread_maxima[tid] = thread_max;
-    const RowSums sums = combine_fast<MODE>(acc, lds);  // its barriers also publish the maxima
-    if (tid < kWave) {
-      const uint32_t bits = kth_maximum(thread_maxima, a.k);
-      if (tid == 0) bar_bits = bits;
-    }
-    const RowSoftmax mine = row_softmax<DT, MODE>(row, g, sums, c_scaled, a.temperature, lds);
-    __syncthreads();
-    const uint32_t bits = bar_bits;
-    const float bar = bits <= ordered_bits(-INFINITY) ? -INFINITY : ordered_value(bits);
-    collect_blocks<DT>(row, g, 0u, block_max, a.shift, bar, thread_max, cand);
-    __syncthreads();
-    int n = cand.count;
-    if (n > kCap || mine.nan) {
-      __syncthreads();
-      if (tid == 0) cand.count = 0;
-      collect_row<DT>(row, g, 0u, a.k, bits != 0u ? ((uint64_t)bits << 32) - 1u : 0ull, cand);
-      n = cand.count;
-    }
-    auto out = [&](uint64_t key, int at) {
-      a.top_ids[row_i * a.k + at] = (int64_t)key_id(key);
-      a.top_logprob[row_i * a.k + at] = logprob_of(ordered_value((uint32_t)(key >> 32)), a.temperature, mine);
-    };
-    if (n <= kBlock) {
-      uint64_t key[1];
-      int rank[1];
-      rank_candidates<1>(cand, n, key, rank);
-      if (tid < n && rank[0] < a.k) out(key[0], rank[0]);
-    } else {
-      keep_best(cand, a.k);
-      if (tid < a.k) out(cand.key[tid], tid);
-    }
-    if (tid == 0) {
-      if (a.logprob != nullptr)
-        a.logprob[row_i] = label >= 0 && label < a.vocab ? logprob_of(x_label, a.temperature, mine) : (label == -100 ? 0.0f : NAN);
-      if (ModeTraits<MODE>::kPlainSet && a.entropy != nullptr) a.entropy[row_i] = (float)mine.entropy;
-      if (a.row_stats != nullptr) *(f32x4*)(a.row_stats + row_i * 4) = f32x4{mine.centre, mine.l2_t, mine.l2_1, mine.ex};
-    }
-    __syncthreads();  // the candidates are read until here
+    collect_row<DT>(row, g, 0u, a.k, bits != 0u ? ((uint64_t)bits << 32) - 1u : 0ull, cand);
+    n = cand.count;
+  }
+  auto out = [&](uint64_t key, int at) {
+    a.top_ids[row_i * a.k + at] = (int64_t)key_id(key);
+    a.top_logprob[row_i * a.k + at] = logprob_of(ordered_value((uint32_t)(key >> 32)), a.temperature, softmax);
+  };
+  if (n <= kBlock) {
+    uint64_t key[1];
+    int rank[1];
+    rank_candidates<1>(cand, n, key, rank);
+    if (tid < n && rank[0] < a.k) out(key[0], rank[0]);
+  } else {
+    keep_best(cand, a.k);
+    if (tid < a.k) out(cand.key[tid], tid);
+  }
+  if (tid == 0) {
+    if (a.logprob != nullptr)
+      a.logprob[row_i] = label >= 0 && label < a.vocab ? logprob_of(x_label, a.temperature, softmax) : (label == -100 ? 0.0f : NAN);
+    if (ModeTraits<MODE>::kPlainSet && a.entropy != nullptr) a.entropy[row_i] = (float)softmax.entropy;
+    if (a.row_stats != nullptr) *(f32x4*)(a.row_stats + row_i * 4) = f32x4{softmax.centre, softmax.l2_t, softmax.l2_1, softmax.ex};
   }
 }
 
@@ -587,55 +666,54 @@ __global__ __launch_bounds__(kBlock) void top_logprobs_bwd_kernel(TopBwdArgs a) 
   __shared__ float lds[kWavesPerBlock];
   const int tid = threadIdx.x;
   const double inv_t = 1.0 / a.temperature;
-  for (int64_t row_i = blockIdx.x; row_i < a.n_rows; row_i += gridDim.x) {
-    const char* row = a.logits + row_i * a.row_stride_bytes;
-    char* out_row = a.grad + row_i * a.grad_stride_bytes;
-    const RowGeom g = row_geom<DT>(row, a.vocab, a.scalar_only != 0);
-    const bool skipped = a.row_mask != nullptr && a.row_mask[row_i] == 0;
-    const bool mine = !skipped && tid < a.k && a.g_top != nullptr;
-    const float gk = mine ? a.g_top[row_i * a.k + tid] : 0.0f;
-    const int64_t id = mine ? a.top_ids[row_i * a.k + tid] : -1;
-    const float w = wave_sum(gk);
-    const bool wave_on = __ballot(gk != 0.0f) != 0ull;  // NaN counts as on
-    if ((tid & (kWave - 1)) == 0) lds[tid / kWave] = w;
-    const bool top_on = __syncthreads_or(wave_on);
-    float sum_top = 0.0f;
+  const int64_t row_i = grid_row();
+  if (row_i >= a.n_rows) return;
+  const char* row = a.logits + row_i * a.row_stride_bytes;
+  char* out_row = a.grad + row_i * a.grad_stride_bytes;
+  const RowGeom g = row_geom<DT>(row, a.vocab, a.scalar_only != 0);
+  const bool skipped = a.row_mask != nullptr && a.row_mask[row_i] == 0;
+  const bool mine = !skipped && tid < a.k && a.g_top != nullptr;
+  const float gk = mine ? a.g_top[row_i * a.k + tid] : 0.0f;
+  const int64_t id = mine ? a.top_ids[row_i * a.k + tid] : -1;
+  const float w = wave_sum(gk);
+  const bool wave_on = __ballot(gk != 0.0f) != 0ull;  // NaN counts as on
+  if ((tid & (kWave - 1)) == 0) lds[tid / kWave] = w;
+  const bool top_on = __syncthreads_or(wave_on);
+  float sum_top = 0.0f;
 #pragma unroll
-    for (int i = 0; i < kWavesPerBlock; ++i) sum_top += lds[i];
+  for (int i = 0; i < kWavesPerBlock; ++i) sum_top += lds[i];
+  __syncthreads();
+  const float glp = a.g_logprob != nullptr ? a.g_logprob[row_i] : 0.0f;
+  const float gh = MODE != kBwdLp ? a.g_entropy[row_i] : 0.0f;
+  if (skipped || (glp == 0.0f && gh == 0.0f && !top_on)) {
+    zero_row<DT>(out_row, g);
+    return;
+  }
+  const f32x4 st = *(const f32x4*)(a.row_stats + row_i * 4);
+  const double all = (double)glp + (double)sum_top;
+  ListGrad<MODE> fn;
+  fn.centre = st[0];
+  fn.cT = (float)(1.4426950408889634 * inv_t);
+  fn.negLT = -st[1];
+  fn.negL1 = -st[2];
+  fn.a_all = -(float)(all * inv_t);
+  fn.onehot = (float)((double)glp * inv_t);
+  fn.gh = gh;
+  fn.k1 = gh * st[3] + (MODE == kBwdBothT1 ? fn.a_all : 0.0f);
+  const int64_t label = a.g_logprob != nullptr ? a.labels[row_i] : -1;
+  fn.set_label(label, a.vocab, g, E::kPerVec);
+  const bool patch = mine && id >= 0 && id < a.vocab;
+  float val = 0.0f;
+  if (patch) {
+    val = E::load1(row + id * E::kSize);
+    fn.one(val, (uint32_t)id);
+    val += (float)((double)gk * inv_t);
+  }
+  if (a.g_top != nullptr) __syncthreads();  // the listed logits are read before any is overwritten
+  traverse_row<DT, true>(row, out_row, g, fn);
+  if (a.g_top != nullptr) {
     __syncthreads();
-    const float glp = a.g_logprob != nullptr ? a.g_logprob[row_i] : 0.0f;
-    const float gh = MODE != kBwdLp ? a.g_entropy[row_i] : 0.0f;
-    if (skipped || (glp == 0.0f && gh == 0.0f && !top_on)) {
-      zero_row<DT>(out_row, g);
-      continue;
-    }
-    const f32x4 st = *(const f32x4*)(a.row_stats + row_i * 4);
-    const double all = (double)glp + (double)sum_top;
-    ListGrad<MODE> fn;
-    fn.centre = st[0];
-    fn.cT = (float)(1.4426950408889634 * inv_t);
-    fn.negLT = -st[1];
-    fn.negL1 = -st[2];
-    fn.a_all = -(float)(all * inv_t);
-    fn.onehot = (float)((double)glp * inv_t);
-    fn.gh = gh;
-    fn.k1 = gh * st[3] + (MODE == kBwdBothT1 ? fn.a_all : 0.0f);
-    const int64_t label = a.g_logprob != nullptr ? a.labels[row_i] : -1;
-    fn.set_label(label, a.vocab, g, E::kPerVec);
-    const bool patch = mine && id >= 0 && id < a.vocab;
-    float val = 0.0f;
-    if (patch) {
-      val = E::load1(row + id * E::kSize);
-      fn.one(val, (uint32_t)id);
-      val += (float)((double)gk * inv_t);
-    }
-    if (a.g_top != nullptr) __syncthreads();  // the listed logits are read before any is overwritten
-    traverse_row<DT, true>(row, out_row, g, fn);
-    if (a.g_top != nullptr) {
-      __syncthreads();
-      if (patch) E::store1(out_row + id * E::kSize, val);
-      __syncthreads();
-    }
+    if (patch) E::store1(out_row + id * E::kSize, val);
   }
 }
 
@@ -645,8 +723,9 @@ static int launch_top_fwd(TopArgs a, hipStream_t stream) {
   const int64_t parts = (a.vocab / Elt<DT>::kPerVec + kBlockVecs * kBlock - 1) / (kBlockVecs * kBlock);
   while ((parts + (1 << a.shift) - 1) >> a.shift > kMaxBlocks) ++a.shift;
   const int64_t blocks = (parts + (1 << a.shift) - 1) >> a.shift;
-  const size_t lds = (size_t)(blocks > 0 ? blocks : 1) * kBlock * sizeof(float);
-  const dim3 grid(grid_for_rows(a.n_rows)), block(kBlock);
+  const size_t maxima = (size_t)blocks * kBlock * sizeof(float), keys = kCap * sizeof(uint64_t);
+  const size_t lds = maxima > keys ? maxima : keys;
+  const dim3 grid = row_grid(a.n_rows), block(kBlock);
   if (a.entropy == nullptr)
     hipLaunchKernelGGL((top_logprobs_fwd_kernel<DT, kLpOnly>), grid, block, lds, stream, a);
   else if (t1)
@@ -659,7 +738,7 @@ static int launch_top_fwd(TopArgs a, hipStream_t stream) {
 
 template <int DT>
 static int launch_top_bwd(const TopBwdArgs& a, hipStream_t stream) {
-  const dim3 grid(grid_for_rows(a.n_rows)), block(kBlock);
+  const dim3 grid = row_grid(a.n_rows), block(kBlock);
   if (a.g_entropy == nullptr)
     hipLaunchKernelGGL((top_logprobs_bwd_kernel<DT, kBwdLp>), grid, block, 0, stream, a);
   else if (a.temperature == 1.0)
