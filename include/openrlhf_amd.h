@@ -165,11 +165,19 @@ int orlhf_logprob_entropy_bwd(const void* logits, void* grad_logits, int dtype, 
  *   row_stats          float [n_rows, 4] or NULL: what orlhf_top_logprobs_bwd needs of the softmax
  * 1 <= k <= 128, k <= vocab. Rows with row_mask 0 are not read: ids -1, everything else 0. No
  * reference counterpart: the alternatives extend openrlhf/models/utils.py:139-163,182-186.
+ *
+ * A launch with too few rows to fill the GPU cuts them into segments, one workgroup each, whose
+ * records go through `workspace` (orlhf_top_logprobs_workspace_bytes; 0: not cut, NULL will do). The
+ * cut depends on the shape only. `tickets`: n_rows int32, all zero, as in
+ * orlhf_logprob_entropy_fwd_split (zero again when the call is done; calls that may overlap need
+ * arrays of their own), or NULL: a second small launch merges the records, with the same bits.
  */
+int64_t orlhf_top_logprobs_workspace_bytes(int dtype, int64_t n_rows, int64_t vocab, int64_t k);
 int orlhf_top_logprobs_fwd(const void* logits, int dtype, int64_t n_rows, int64_t vocab,
                            int64_t row_stride, const int64_t* labels, double temperature, int64_t k,
                            float* logprob, float* entropy, float* top_logprob, int64_t* top_ids,
-                           float* row_stats, const uint8_t* row_mask, orlhf_stream_t stream);
+                           float* row_stats, const uint8_t* row_mask, void* workspace,
+                           int64_t workspace_bytes, int32_t* tickets, orlhf_stream_t stream);
 
 /*
  * Its backward, written in the logits dtype: orlhf_logprob_entropy_bwd's gradient plus

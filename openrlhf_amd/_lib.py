@@ -83,7 +83,8 @@ SIGNATURES = {
     "orlhf_logprob_entropy_bwd": (c_int, [P, P, c_int, I64, I64, I64, I64, P, c_double, P, P, P, P, P]),
     "orlhf_logprob_entropy_fwd_bwd_max_vocab": (I64, [c_int]),
     "orlhf_logprob_entropy_fwd_bwd": (c_int, [P, P, c_int, I64, I64, I64, I64, P, c_double, P, P, P, P, P, P]),
-    "orlhf_top_logprobs_fwd": (c_int, [P, c_int, I64, I64, I64, P, c_double, I64, P, P, P, P, P, P, P]),
+    "orlhf_top_logprobs_workspace_bytes": (I64, [c_int, I64, I64, I64]),
+    "orlhf_top_logprobs_fwd": (c_int, [P, c_int, I64, I64, I64, P, c_double, I64, P, P, P, P, P, P, P, I64, P, P]),
     "orlhf_top_logprobs_bwd": (c_int, [P, P, c_int, I64, I64, I64, I64, P, c_double, I64, P, P, P, P, P, P, P]),
     "orlhf_lmhead_workspace_bytes": (I64, [I64, I64, I64, I64, c_int]),
     "orlhf_lmhead_logprob_entropy_fwd": (c_int, [P, P, c_int, I64, I64, I64, I64, I64, P, c_double, P, P, P, P, I64, I64,

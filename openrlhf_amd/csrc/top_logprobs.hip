@@ -9,7 +9,7 @@
 // means "ranked before", and a NaN (which has no order) ranks before everything.
 #include <type_traits>
 
-#include "vocab_rows.h"
+#include "list_rows.h"
 
 namespace orlhf {
 
@@ -34,7 +34,9 @@ struct Candidates {
   int& count;
 };
 
-// How many of the n candidates rank before each of this thread's (at threadIdx.x + i * kBlock).
+// How many of the n candidates rank before each of this thread's (at threadIdx.x + i * kBlock). The
+// candidates are read eight at a time, all lanes the same: a broadcast.
+typedef uint64_t u64x2 __attribute__((ext_vector_type(2)));
 template <int MINE>
 __device__ __forceinline__ void rank_candidates(const Candidates& c, int n, uint64_t (&mine)[MINE], int (&rank)[MINE]) {
 #pragma unroll
@@ -44,27 +46,42 @@ __device__ __forceinline__ void rank_candidates(const Candidates& c, int n, uint
     rank[i] = 0;
   }
   if ((int)(threadIdx.x & ~(kWave - 1u)) >= n) return;  // a wave without a candidate
-#pragma unroll 4
-  for (int j = 0; j < n; ++j) {
-    const uint64_t other = c.key[j];
+  auto count = [&](uint64_t other) {
 #pragma unroll
     for (int i = 0; i < MINE; ++i) rank[i] += other > mine[i] ? 1 : 0;
+  };
+  int j = 0;
+  for (; j + 8 <= n; j += 8) {
+    u64x2 two[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) two[q] = *(const u64x2*)(c.key + j + 2 * q);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) count(two[q][0]), count(two[q][1]);
+  }
+  for (; j < n; ++j) count(c.key[j]);
+}
+
+template <int MINE>
+__device__ __forceinline__ void sort_best(const Candidates& c, int n, int k) {
+  uint64_t mine[MINE];
+  int rank[MINE];
+  rank_candidates<MINE>(c, n, mine, rank);
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < MINE; ++i) {
+    const int at = (int)threadIdx.x + i * kBlock;
+    if (at < n && rank[i] < k) c.key[rank[i]] = mine[i];
   }
 }
 
 // Keeps the k best candidates, sorted, and returns the k-th (0 while there are fewer). The whole
 // workgroup calls it with the candidates in place behind a barrier; another one ends it.
 __device__ __forceinline__ uint64_t keep_best(const Candidates& c, int k) {
-  constexpr int kMine = kCap / kBlock;
   const int n = c.count;
-  uint64_t mine[kMine];
-  int rank[kMine];
-  rank_candidates<kMine>(c, n, mine, rank);
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < kMine; ++i) {
-    const int at = (int)threadIdx.x + i * kBlock;
-    if (at < n && rank[i] < k) c.key[rank[i]] = mine[i];
+  if (n <= 2 * kBlock) {
+    sort_best<2>(c, n, k);
+  } else {
+    sort_best<kCap / kBlock>(c, n, k);
   }
   if (threadIdx.x == 0) c.count = n < k ? n : k;
   __syncthreads();
@@ -121,14 +138,6 @@ __device__ __forceinline__ void collect_row(const char* row, const RowGeom& g, u
   __syncthreads();
 }
 
-// One workgroup per row and no loop over rows in the kernels: a loop makes the compiler keep the
-// constants of the whole body (of the logarithms above all) in registers, 20 to 30 per lane.
-constexpr int64_t kGridX = 1 << 20;
-inline dim3 row_grid(int64_t n_rows) {
-  return dim3((unsigned)(n_rows < kGridX ? n_rows : kGridX), (unsigned)((n_rows + kGridX - 1) / kGridX));
-}
-__device__ __forceinline__ int64_t grid_row() { return (int64_t)blockIdx.y * kGridX + blockIdx.x; }
-
 struct TopArgs {
   const char* logits;
   int64_t n_rows, vocab, row_stride_bytes;
@@ -139,6 +148,9 @@ struct TopArgs {
   int64_t* top_ids;
   const uint8_t* row_mask;
   int shift;  // of the selection's blocks
+  ListSplit split;
+  uint64_t* records;  // split rows: kTotalsWords + k words per (row, segment)
+  int32_t* tickets;   // split rows: one per row, zero between launches; NULL: a second launch merges
 };
 
 __device__ __forceinline__ void write_skipped_row(const TopArgs& a, int64_t row_i) {
@@ -151,193 +163,6 @@ __device__ __forceinline__ void write_skipped_row(const TopArgs& a, int64_t row_
     if (a.entropy != nullptr) a.entropy[row_i] = 0.0f;
     if (a.row_stats != nullptr) *(f32x4*)(a.row_stats + row_i * 4) = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   }
-}
-
-// The softmax of a row as what its outputs and its backward need: base + log_sum is the
-// log-sum-exp of x / T (kept apart: base may be so large that the sum would be lost in it), `centre`
-// a logit near base * T that every later difference starts from, entropy and E[x] - centre those of
-// the unscaled logits.
-struct RowSoftmax {
-  double base, log_sum, entropy;
-  float centre, l2_t, l2_1, ex;  // the backward's statistics: softmax(x / T) = 2^((x - centre) cT - l2_t)
-};
-
-// Fast pass: per wave sums against its reference, folded over the workgroup.
-template <int MODE>
-__device__ __forceinline__ RowSums combine_fast(const FastAcc<MODE>& acc, float (*lds)[8]) {
-  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-  float st, s, t;
-  acc.fold(st, s, t);
-  st = wave_sum(st);
-  s = wave_sum(s);
-  t = wave_sum(t);
-  if (lane == 0) {
-    lds[wave][0] = -acc.negMT;
-    lds[wave][1] = st;
-    lds[wave][2] = -acc.negM1;
-    lds[wave][3] = s;
-    lds[wave][4] = t;
-  }
-  __syncthreads();
-  RowSums r;
-  r.MT = lds[0][0], r.M1 = lds[0][2];
-#pragma unroll
-  for (int w = 1; w < kWavesPerBlock; ++w) {
-    r.MT = fmaxf(r.MT, lds[w][0]);
-    r.M1 = fmaxf(r.M1, lds[w][2]);
-  }
-  r.sT = r.s1 = r.t1 = 0.0f;
-#pragma unroll
-  for (int w = 0; w < kWavesPerBlock; ++w) {
-    r.sT = fmaf(lds[w][1], fast_exp2(lds[w][0] - r.MT), r.sT);
-    const float q = fast_exp2(lds[w][2] - r.M1);
-    r.s1 = fmaf(lds[w][3], q, r.s1);
-    r.t1 = fmaf(lds[w][4], q, r.t1);
-  }
-  __syncthreads();
-  return r;
-}
-
-// Rows whose fast sums are not usable (an element some 88 nats above the references, logits at the
-// lowest values of their type, inf, NaN) or would lose digits (references so far from 0 that the
-// roundings of x c, which grow with |x|, reach 2^-16 and the entropy's with it): the exact maximum
-// first, then sums of the differences to it.
-constexpr float kFarReference = 256.0f;  // log2 units
-
-struct MaxAcc {
-  float m;
-  bool nan;
-  __device__ __forceinline__ void one(float& x, uint32_t) {
-    m = fmaxf(m, x);
-    nan = nan || x != x;
-  }
-  template <int N>
-  __device__ __forceinline__ void vec(float (&x)[N], uint32_t v) {
-#pragma unroll
-    for (int j = 0; j < N; ++j) one(x[j], v);
-  }
-};
-template <int MODE>
-struct ExactAcc {
-  float m, cT, c1, sT, s1, t1;  // t1: sum of e (x - m); an element of weight 0 adds 0, also at -inf
-  __device__ __forceinline__ void one(float& x, uint32_t) {
-    const float d = x == m ? 0.0f : x - m;  // also for m = +-inf
-    if (ModeTraits<MODE>::kScaledSet) sT += fast_exp2(d * cT);
-    if (ModeTraits<MODE>::kPlainSet) {
-      const float e = fast_exp2(d * c1);
-      s1 += e;
-      t1 += e > 0.0f ? e * d : 0.0f;
-    }
-  }
-  template <int N>
-  __device__ __forceinline__ void vec(float (&x)[N], uint32_t v) {
-#pragma unroll
-    for (int j = 0; j < N; ++j) one(x[j], v);
-  }
-};
-
-// The sums of a row in the form that finish_row takes: of 2^((x - ref) c), with the reference in log2
-// units after the fast pass and as a logit after the exact one.
-struct RowTotals {
-  float ref_t, ref_1;
-  double sT, s1, t1;  // t1: sum of e x (fast) or of e (x - ref) (exact)
-  bool fast, nan;
-};
-
-template <int MODE>
-__device__ __forceinline__ bool fast_usable(const RowSums& s) {
-  using MT = ModeTraits<MODE>;
-  bool ok = true;
-  if (MT::kScaledSet) ok = ok && sums_usable(s.sT) && fabsf(s.MT) < kFarReference;
-  if (MT::kPlainSet) ok = ok && sums_usable(s.s1) && fabsf(s.t1) < INFINITY && fabsf(s.M1) < kFarReference;
-  return ok;
-}
-
-// One vector per step: what only rare rows run must not cost the others their registers.
-template <int DT, typename F>
-__device__ __forceinline__ void walk_row(const char* row, const RowGeom& g, F& f) {
-  using E = Elt<DT>;
-  const uint32_t tid = threadIdx.x;
-  const char* body = row + g.head * E::kSize;
-#pragma unroll 1
-  for (uint32_t v = tid; v < g.nvec; v += kBlock) {
-    float x[E::kPerVec];
-    E::unpack(*(const u32x4*)(body + v * 16u), x);
-    f.vec(x, v);
-  }
-  if (tid < g.head + g.tail) {
-    const uint32_t e = tid < g.head ? tid : g.nvec * E::kPerVec + tid;
-    float x = E::load1(row + e * E::kSize);
-    f.one(x, e);
-  }
-}
-
-template <int DT, int MODE>
-__device__ __forceinline__ RowTotals exact_totals(const char* row, const RowGeom& g, float c_scaled, float (*lds)[8]) {
-  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-  MaxAcc top{-INFINITY, false};
-  walk_row<DT>(row, g, top);
-  const float m_w = wave_max(top.m);
-  const bool nan_w = __ballot(top.nan) != 0ull;
-  if (lane == 0) {
-    lds[wave][0] = m_w;
-    lds[wave][1] = nan_w ? 1.0f : 0.0f;
-  }
-  __syncthreads();
-  float m = lds[0][0], nans = lds[0][1];
-#pragma unroll
-  for (int w = 1; w < kWavesPerBlock; ++w) {
-    m = fmaxf(m, lds[w][0]);
-    nans += lds[w][1];
-  }
-  __syncthreads();
-  ExactAcc<MODE> acc{m, c_scaled, kLog2e, 0.0f, 0.0f, 0.0f};
-  walk_row<DT>(row, g, acc);
-  const float st = wave_sum(acc.sT), s = wave_sum(acc.s1), t = wave_sum(acc.t1);
-  if (lane == 0) {
-    lds[wave][0] = st;
-    lds[wave][1] = s;
-    lds[wave][2] = t;
-  }
-  __syncthreads();
-  RowTotals r = {m, m, 0.0, 0.0, 0.0, false, nans != 0.0f};
-#pragma unroll
-  for (int w = 0; w < kWavesPerBlock; ++w) {
-    r.sT += (double)lds[w][0];
-    r.s1 += (double)lds[w][1];
-    r.t1 += (double)lds[w][2];
-  }
-  __syncthreads();
-  if (r.nan || m == -INFINITY) r.sT = r.s1 = NAN;
-  if (m == INFINITY) r.t1 = NAN;
-  return r;
-}
-
-template <int MODE>
-__device__ __forceinline__ RowSoftmax finish_row(const RowTotals& t, double temperature) {
-  using MT = ModeTraits<MODE>;
-  RowSoftmax r;
-  const double scale = MT::kScaledSet ? temperature : 1.0;  // one set serves both where T = 1
-  const double base_1 = t.fast ? (double)t.ref_1 * kLn2d : (double)t.ref_1;
-  double log_1 = 0.0, ex = 0.0;  // of the unscaled logits; ex = E[x] - base_1
-  if (MT::kPlainSet) {
-    log_1 = log(t.s1);
-    ex = t.t1 / t.s1 - (t.fast ? base_1 : 0.0);
-  }
-  r.base = MT::kScaledSet ? (t.fast ? (double)t.ref_t * kLn2d : (double)t.ref_t / temperature) : base_1;
-  r.log_sum = MT::kScaledSet ? log(t.sT) : log_1;
-  const double at = r.base * scale;
-  r.centre = (float)at;
-  r.l2_t = (float)((r.log_sum + (at - (double)r.centre) / scale) * 1.4426950408889634);
-  r.entropy = log_1 - ex;
-  const double rest = base_1 - (double)r.centre;
-  r.l2_1 = MT::kPlainSet ? (float)((log_1 + rest) * 1.4426950408889634) : 0.0f;
-  r.ex = MT::kPlainSet ? (float)(ex + rest) : 0.0f;
-  return r;
-}
-
-__device__ __forceinline__ float logprob_of(float x, double temperature, const RowSoftmax& r) {
-  return (float)(((double)x / temperature - r.base) - r.log_sum);
 }
 
 // ---------------------------------------------------------------- selection
@@ -441,14 +266,11 @@ __device__ __forceinline__ float stream_row(const char* row, const RowGeom& g, f
   return thread_max;
 }
 
-// The largest value of 16 leading bits that at least k of the 256 maxima reach, as ordered bits: one
-// wave, four maxima per lane, one counting step per bit.
-__device__ __forceinline__ uint32_t kth_maximum(const float* thread_max, int k) {
+// The largest value of 16 leading bits that at least k of the 256 values reach: one wave, four values
+// per lane, one counting step per bit.
+__device__ __forceinline__ uint32_t kth_largest(const uint32_t* values, int k) {
   const int lane = threadIdx.x & (kWave - 1);
-  const f32x4 m = *(const f32x4*)(thread_max + lane * 4);
-  uint32_t o[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) o[i] = ordered_bits(m[i]);
+  const u32x4 o = *(const u32x4*)(values + lane * 4);
   uint32_t found = 0;
 #pragma unroll
   for (int bit = 31; bit >= 16; --bit) {
@@ -525,63 +347,20 @@ __device__ __forceinline__ void collect_blocks(const char* row, const RowGeom& g
   }
 }
 
-template <int DT, int MODE>
-__global__ __launch_bounds__(kBlock) void top_logprobs_fwd_kernel(TopArgs a) {
-  using E = Elt<DT>;
-  __shared__ float lds[kWavesPerBlock][8];
-  __shared__ int n_cand;
-  __shared__ BlockList list;
-  __shared__ alignas(16) float thread_maxima[kBlock];
-  __shared__ uint32_t bar_bits;
-  __shared__ RowSoftmax softmax;
-  extern __shared__ uint64_t shared[];  // block maxima while the row streams by, candidates afterwards
-  float* const block_max = (float*)shared;
-  const Candidates cand = {shared, n_cand};
-  const int tid = threadIdx.x;
-  const float c_scaled = (float)(1.4426950408889634 / a.temperature);
-  const int64_t row_i = grid_row();
-  if (row_i >= a.n_rows) return;
-  if (a.row_mask != nullptr && a.row_mask[row_i] == 0) {
-    write_skipped_row(a, row_i);
-    return;
-  }
-  const char* row = a.logits + row_i * a.row_stride_bytes;
-  const RowGeom g = row_geom<DT>(row, a.vocab, false);
-  if (tid == 0) n_cand = list.count = 0;
-  // the label and its logit are asked for now and used by the row's last instructions
-  int64_t label = -1;
-  float x_label = 0.0f;
-  if (a.logprob != nullptr && tid == 0) {
-    label = a.labels[row_i];
-    if (label >= 0 && label < a.vocab) x_label = E::load1(row + label * E::kSize);
-  }
-  FastAcc<MODE> acc;
-  const float thread_max = stream_row<DT, MODE>(row, g, c_scaled, acc, block_max, a.shift);
-  thread_maxima[tid] = thread_max;
-  const RowSums sums = combine_fast<MODE>(acc, lds);  // its barriers also publish the maxima
-  const bool fast = fast_usable<MODE>(sums);
-  RowTotals totals = {sums.MT, sums.M1, sums.sT, sums.s1, sums.t1, true, false};
-  if (!fast) totals = exact_totals<DT, MODE>(row, g, c_scaled, lds);
-  const bool nan = totals.nan;
-  if (tid < kWave) {  // one wave finds the bar, another takes the logarithms
-    const uint32_t bits = kth_maximum(thread_maxima, a.k);
-    if (tid == 0) bar_bits = bits;
-  } else if (tid < 2 * kWave) {
-    const RowSoftmax r = finish_row<MODE>(totals, a.temperature);
-    if (tid == kWave) softmax = r;
-  }
-  __syncthreads();
-  const uint32_t bits = bar_bits;
-  const float bar = bits <= ordered_bits(-INFINITY) ? -INFINITY : ordered_value(bits);
-  collect_blocks<DT>(row, g, 0u, block_max, a.shift, bar, thread_max, list, cand);
-  __syncthreads();
-  int n = cand.count;
-  if (n > kCap || list.count > kListed || nan) {
-    __syncthreads();
-    if (tid == 0) cand.count = 0;
-    collect_row<DT>(row, g, 0u, a.k, bits != 0u ? ((uint64_t)bits << 32) - 1u : 0ull, cand);
-    n = cand.count;
-  }
+struct TopShared {
+  float lds[kWavesPerBlock][8];
+  int n_cand;
+  BlockList list;
+  alignas(16) uint32_t best[kBlock];  // ordered bits of the largest value each thread has seen
+  uint32_t bar_bits;
+  RowSoftmax softmax;
+};
+
+// The row's outputs from its candidates (in place behind a barrier) and its softmax.
+template <int MODE>
+__device__ __forceinline__ void write_row(const TopArgs& a, int64_t row_i, const Candidates& cand, int64_t label,
+                                          float x_label, const RowSoftmax& softmax) {
+  const int tid = threadIdx.x, n = cand.count;
   auto out = [&](uint64_t key, int at) {
     a.top_ids[row_i * a.k + at] = (int64_t)key_id(key);
     a.top_logprob[row_i * a.k + at] = logprob_of(ordered_value((uint32_t)(key >> 32)), a.temperature, softmax);
@@ -603,6 +382,140 @@ __global__ __launch_bounds__(kBlock) void top_logprobs_fwd_kernel(TopArgs a) {
   }
 }
 
+// A cut row from its segments' records: the k best of their lists, the merged softmax.
+template <int MODE, bool FRESH>
+__device__ __forceinline__ void merge_top_row(const TopArgs& a, int64_t row_i, const Candidates& cand, TopShared& sh) {
+  const int tid = threadIdx.x, stride = kTotalsWords + a.k, total = a.split.n * a.k;
+  const uint64_t* rec = a.records + row_i * a.split.n * stride;
+  const int64_t label = a.logprob != nullptr ? a.labels[row_i] : -1;
+  float x_label = 0.0f;
+  if (tid < kWave) {
+    const int at = label >= 0 && label < a.vocab ? (int)(label / a.split.seg_elems) : -1;
+    const RowTotals t = merge_totals<FRESH>(rec, stride, a.split.n, at, x_label);
+    const RowSoftmax r = finish_row<MODE>(t, a.temperature);
+    if (tid == 0) sh.softmax = r;
+  }
+  auto key_at = [&](int i) { return get64<FRESH>(rec + (int64_t)(i / a.k) * stride + kTotalsWords + i % a.k); };
+  // a bar as in the rows themselves: the k-th largest of the threads' best keys (absent keys are 0)
+  uint64_t best = 0;
+#pragma unroll 1
+  for (int i = tid; i < total; i += kBlock) {
+    const uint64_t key = key_at(i);
+    if (i < kCap) cand.key[i] = key;
+    best = key > best ? key : best;
+  }
+  sh.best[tid] = (uint32_t)(best >> 32);
+  if (tid == 0) sh.n_cand = 0;
+  __syncthreads();
+  if (tid < kWave) {
+    const uint32_t bits = kth_largest(sh.best, a.k);
+    if (tid == 0) sh.bar_bits = bits;
+  }
+  __syncthreads();
+  const uint32_t bits = sh.bar_bits;
+  const uint64_t least = bits != 0u ? ((uint64_t)bits << 32) - 1u : 0ull;
+  uint64_t mine[kCap / kBlock];
+#pragma unroll
+  for (int i = 0; i < kCap / kBlock; ++i) mine[i] = tid + i * kBlock < total ? cand.key[tid + i * kBlock] : 0ull;
+  __syncthreads();
+  if (total <= kCap) {
+#pragma unroll
+    for (int i = 0; i < kCap / kBlock; ++i)
+      if (mine[i] > least) cand.key[atomicAdd(&sh.n_cand, 1)] = mine[i];
+  } else {
+    uint64_t above = least;
+#pragma unroll 1
+    for (int i = tid; i - tid < total; i += kBlock) push_round(cand, i < total ? key_at(i) : 0ull, a.k, above);
+  }
+  __syncthreads();
+  write_row<MODE>(a, row_i, cand, label, x_label, sh.softmax);
+}
+
+template <int DT, int MODE>
+__global__ __launch_bounds__(kBlock) void top_logprobs_fwd_kernel(TopArgs a) {
+  using E = Elt<DT>;
+  __shared__ TopShared sh;
+  extern __shared__ uint64_t shared[];  // block maxima while the row streams by, candidates afterwards
+  float* const block_max = (float*)shared;
+  const Candidates cand = {shared, sh.n_cand};
+  const int tid = threadIdx.x;
+  const Segment seg = segment_of(grid_row(), a.split, a.vocab);
+  const int64_t row_i = seg.row;
+  if (row_i >= a.n_rows) return;
+  if (a.row_mask != nullptr && a.row_mask[row_i] == 0) {
+    if (seg.index == 0) write_skipped_row(a, row_i);
+    return;
+  }
+  const char* row = a.logits + row_i * a.row_stride_bytes + (int64_t)seg.first * E::kSize;
+  const RowGeom g = row_geom<DT>(row, seg.len, false);
+  if (tid == 0) sh.n_cand = sh.list.count = 0;
+  // the label and its logit are asked for now and used by the row's last instructions
+  int64_t label = -1;
+  float x_label = 0.0f;
+  if (a.logprob != nullptr && tid == 0) {
+    label = a.labels[row_i];
+    const int64_t at = label - (int64_t)seg.first;
+    if (at >= 0 && at < seg.len) x_label = E::load1(row + at * E::kSize);
+  }
+  FastAcc<MODE> acc;
+  const float thread_max = stream_row<DT, MODE>(row, g, (float)(1.4426950408889634 / a.temperature), acc, block_max, a.shift);
+  sh.best[tid] = ordered_bits(thread_max);
+  const RowSums sums = combine_fast<MODE>(acc, sh.lds);  // its barriers also publish the maxima
+  RowTotals totals;
+  if (fast_usable<MODE>(sums)) {
+    totals = fast_totals<MODE>(sums);
+  } else {
+    totals = exact_totals<DT, MODE>(row, g, EveryElement{}, a.temperature, sh.lds);
+  }
+  const bool nan = totals.nan;
+  if (tid < kWave) {  // one wave finds the bar, another takes the logarithms
+    const uint32_t bits = kth_largest(sh.best, a.k);
+    if (tid == 0) sh.bar_bits = bits;
+  } else if (tid < 2 * kWave && a.split.n == 1) {
+    const RowSoftmax r = finish_row<MODE>(totals, a.temperature);
+    if (tid == kWave) sh.softmax = r;
+  }
+  __syncthreads();
+  const uint32_t bits = sh.bar_bits;
+  const float bar = bits <= ordered_bits(-INFINITY) ? -INFINITY : ordered_value(bits);
+  collect_blocks<DT>(row, g, seg.first, block_max, a.shift, bar, thread_max, sh.list, cand);
+  __syncthreads();
+  int n = cand.count;
+  if (n > kCap || sh.list.count > kListed || nan) {
+    __syncthreads();
+    if (tid == 0) sh.n_cand = 0;
+    collect_row<DT>(row, g, seg.first, a.k, bits != 0u ? ((uint64_t)bits << 32) - 1u : 0ull, cand);
+    n = cand.count;
+  }
+  if (a.split.n == 1) {
+    write_row<MODE>(a, row_i, cand, label, x_label, sh.softmax);
+    return;
+  }
+  uint64_t* rec = a.records + (row_i * a.split.n + seg.index) * (kTotalsWords + a.k);
+  if (n > kBlock) {
+    keep_best(cand, a.k);
+    n = cand.count;
+  }
+  uint64_t key[1];
+  int rank[1];
+  rank_candidates<1>(cand, n, key, rank);
+  if (tid < n && rank[0] < a.k) put64(rec + kTotalsWords + rank[0], key[0]);
+  if (tid >= n && tid < a.k) put64(rec + kTotalsWords + tid, 0ull);
+  if (tid == 0) put_totals(rec, totals, x_label);
+  if (a.tickets != nullptr && last_segment(a.tickets + row_i, a.split.n)) merge_top_row<MODE, true>(a, row_i, cand, sh);
+}
+
+// The merge as a launch of its own, for callers without tickets.
+template <int MODE>
+__global__ __launch_bounds__(kBlock) void top_logprobs_merge_kernel(TopArgs a) {
+  __shared__ TopShared sh;
+  __shared__ uint64_t keys[kCap];
+  const int64_t row_i = grid_row();
+  if (row_i >= a.n_rows || (a.row_mask != nullptr && a.row_mask[row_i] == 0)) return;
+  const Candidates cand = {keys, sh.n_cand};
+  merge_top_row<MODE, false>(a, row_i, cand, sh);
+}
+
 // ---------------------------------------------------------------- backward
 struct TopBwdArgs {
   const char* logits;
@@ -614,46 +527,7 @@ struct TopBwdArgs {
   const float *g_logprob, *g_entropy, *g_top, *row_stats;  // gradients may be NULL: zero
   const uint8_t* row_mask;
   int scalar_only;
-};
-
-// Gradient of one element from the saved statistics. d = x - centre instead of x: the exponent then
-// carries the rounding of a difference, not of two large numbers, and a row at the lowest values of
-// its type is an ordinary row. The lower bound on d keeps 0 * d at 0 for masked logits.
-template <int MODE>
-struct ListGrad {
-  float centre, cT, negLT, negL1;
-  float a_all;   // -(sum of the upstream gradients of all log-probs) / T
-  float gh, k1;  // entropy term p (k1 - gh d), k1 = gh (E[x] - centre) (+ a_all where T = 1 shares the softmax)
-  float onehot;
-  uint32_t label_vec, label_lane, label_elem;
-  __device__ __forceinline__ float elem(float x) const {
-    const float d = fmaxf(x - centre, -1.0e30f);
-    if (MODE == kBwdLp) return fast_exp2(fmaf(d, cT, negLT)) * a_all;
-    if (MODE == kBwdBothT1) return fast_exp2(fmaf(d, cT, negLT)) * fmaf(-gh, d, k1);
-    return fmaf(fast_exp2(fmaf(d, cT, negLT)), a_all, fast_exp2(fmaf(d, kLog2e, negL1)) * fmaf(-gh, d, k1));
-  }
-  __device__ __forceinline__ void one(float& x, uint32_t e) const {
-    x = elem(x);
-    if (e == label_elem) x += onehot;
-  }
-  template <int N>
-  __device__ __forceinline__ void vec(float (&x)[N], uint32_t v) const {
-#pragma unroll
-    for (int j = 0; j < N; ++j) x[j] = elem(x[j]);
-    if (v == label_vec) {
-#pragma unroll
-      for (int j = 0; j < N; ++j) x[j] += (uint32_t)j == label_lane ? onehot : 0.0f;
-    }
-  }
-  __device__ __forceinline__ void set_label(int64_t label, int64_t vocab, const RowGeom& g, int epv) {
-    label_vec = label_lane = label_elem = 0xffffffffu;
-    if (label < 0 || label >= vocab) return;
-    label_elem = (uint32_t)label;
-    if (label_elem >= g.head && label_elem < g.head + g.nvec * (uint32_t)epv) {
-      label_vec = (label_elem - g.head) / (uint32_t)epv;
-      label_lane = (label_elem - g.head) % (uint32_t)epv;
-    }
-  }
+  ListSplit split;
 };
 
 // grad_j = [ g_lp 1(j = label) + sum_k g_k 1(j = id_k) - (g_lp + sum_k g_k) softmax(x / T)_j ] / T
@@ -666,15 +540,16 @@ __global__ __launch_bounds__(kBlock) void top_logprobs_bwd_kernel(TopBwdArgs a) 
   __shared__ float lds[kWavesPerBlock];
   const int tid = threadIdx.x;
   const double inv_t = 1.0 / a.temperature;
-  const int64_t row_i = grid_row();
+  const Segment seg = segment_of(grid_row(), a.split, a.vocab);
+  const int64_t row_i = seg.row;
   if (row_i >= a.n_rows) return;
-  const char* row = a.logits + row_i * a.row_stride_bytes;
-  char* out_row = a.grad + row_i * a.grad_stride_bytes;
-  const RowGeom g = row_geom<DT>(row, a.vocab, a.scalar_only != 0);
+  const char* row = a.logits + row_i * a.row_stride_bytes + (int64_t)seg.first * E::kSize;
+  char* out_row = a.grad + row_i * a.grad_stride_bytes + (int64_t)seg.first * E::kSize;
+  const RowGeom g = row_geom<DT>(row, seg.len, a.scalar_only != 0);
   const bool skipped = a.row_mask != nullptr && a.row_mask[row_i] == 0;
   const bool mine = !skipped && tid < a.k && a.g_top != nullptr;
   const float gk = mine ? a.g_top[row_i * a.k + tid] : 0.0f;
-  const int64_t id = mine ? a.top_ids[row_i * a.k + tid] : -1;
+  const int64_t id = mine ? a.top_ids[row_i * a.k + tid] - (int64_t)seg.first : -1;  // within the segment
   const float w = wave_sum(gk);
   const bool wave_on = __ballot(gk != 0.0f) != 0ull;  // NaN counts as on
   if ((tid & (kWave - 1)) == 0) lds[tid / kWave] = w;
@@ -701,8 +576,8 @@ __global__ __launch_bounds__(kBlock) void top_logprobs_bwd_kernel(TopBwdArgs a) 
   fn.gh = gh;
   fn.k1 = gh * st[3] + (MODE == kBwdBothT1 ? fn.a_all : 0.0f);
   const int64_t label = a.g_logprob != nullptr ? a.labels[row_i] : -1;
-  fn.set_label(label, a.vocab, g, E::kPerVec);
-  const bool patch = mine && id >= 0 && id < a.vocab;
+  fn.set_label(label >= 0 && label < a.vocab ? label - (int64_t)seg.first : -1, seg.len, g, E::kPerVec);
+  const bool patch = mine && id >= 0 && id < seg.len;
   float val = 0.0f;
   if (patch) {
     val = E::load1(row + id * E::kSize);
@@ -717,28 +592,33 @@ __global__ __launch_bounds__(kBlock) void top_logprobs_bwd_kernel(TopBwdArgs a) 
   }
 }
 
-template <int DT>
-static int launch_top_fwd(TopArgs a, hipStream_t stream) {
-  const bool t1 = a.temperature == 1.0;
-  const int64_t parts = (a.vocab / Elt<DT>::kPerVec + kBlockVecs * kBlock - 1) / (kBlockVecs * kBlock);
-  while ((parts + (1 << a.shift) - 1) >> a.shift > kMaxBlocks) ++a.shift;
-  const int64_t blocks = (parts + (1 << a.shift) - 1) >> a.shift;
-  const size_t maxima = (size_t)blocks * kBlock * sizeof(float), keys = kCap * sizeof(uint64_t);
-  const size_t lds = maxima > keys ? maxima : keys;
-  const dim3 grid = row_grid(a.n_rows), block(kBlock);
-  if (a.entropy == nullptr)
-    hipLaunchKernelGGL((top_logprobs_fwd_kernel<DT, kLpOnly>), grid, block, lds, stream, a);
-  else if (t1)
-    hipLaunchKernelGGL((top_logprobs_fwd_kernel<DT, kBothT1>), grid, block, lds, stream, a);
-  else
-    hipLaunchKernelGGL((top_logprobs_fwd_kernel<DT, kBothT>), grid, block, lds, stream, a);
+template <int DT, int MODE>
+static int launch_top_mode(const TopArgs& a, size_t lds, hipStream_t stream) {
+  hipLaunchKernelGGL((top_logprobs_fwd_kernel<DT, MODE>), row_grid(a.n_rows * a.split.n), dim3(kBlock), lds, stream, a);
   ORLHF_CHECK_LAUNCH("orlhf_top_logprobs_fwd");
+  if (a.split.n > 1 && a.tickets == nullptr) {
+    hipLaunchKernelGGL((top_logprobs_merge_kernel<MODE>), row_grid(a.n_rows), dim3(kBlock), 0, stream, a);
+    ORLHF_CHECK_LAUNCH("orlhf_top_logprobs_fwd(merge)");
+  }
   return ORLHF_OK;
 }
 
 template <int DT>
+static int launch_top_fwd(TopArgs a, hipStream_t stream) {
+  const int64_t len = a.split.n == 1 ? a.vocab : (int64_t)a.split.seg_elems;
+  const int64_t parts = (len / Elt<DT>::kPerVec + kBlockVecs * kBlock - 1) / (kBlockVecs * kBlock);
+  while ((parts + (1 << a.shift) - 1) >> a.shift > kMaxBlocks) ++a.shift;
+  const int64_t blocks = (parts + (1 << a.shift) - 1) >> a.shift;
+  const size_t maxima = (size_t)blocks * kBlock * sizeof(float), keys = kCap * sizeof(uint64_t);
+  const size_t lds = maxima > keys ? maxima : keys;
+  if (a.entropy == nullptr) return launch_top_mode<DT, kLpOnly>(a, lds, stream);
+  if (a.temperature == 1.0) return launch_top_mode<DT, kBothT1>(a, lds, stream);
+  return launch_top_mode<DT, kBothT>(a, lds, stream);
+}
+
+template <int DT>
 static int launch_top_bwd(const TopBwdArgs& a, hipStream_t stream) {
-  const dim3 grid = row_grid(a.n_rows), block(kBlock);
+  const dim3 grid = row_grid(a.n_rows * a.split.n), block(kBlock);
   if (a.g_entropy == nullptr)
     hipLaunchKernelGGL((top_logprobs_bwd_kernel<DT, kBwdLp>), grid, block, 0, stream, a);
   else if (a.temperature == 1.0)
@@ -765,10 +645,17 @@ static int check_top(const char* what, int dtype, int64_t n_rows, int64_t vocab,
 
 using namespace orlhf;
 
+extern "C" int64_t orlhf_top_logprobs_workspace_bytes(int dtype, int64_t n_rows, int64_t vocab, int64_t k) {
+  if (n_rows <= 0 || vocab <= 0 || vocab >= (1ll << 29) || k < 1 || k > kMaxTop) return 0;
+  const ListSplit split = list_split(n_rows, vocab, dtype == ORLHF_F32 ? 4 : 2);
+  return split.n > 1 ? n_rows * split.n * (kTotalsWords + k) * (int64_t)sizeof(uint64_t) : 0;
+}
+
 extern "C" int orlhf_top_logprobs_fwd(const void* logits, int dtype, int64_t n_rows, int64_t vocab, int64_t row_stride,
                                       const int64_t* labels, double temperature, int64_t k, float* logprob,
                                       float* entropy, float* top_logprob, int64_t* top_ids, float* row_stats,
-                                      const uint8_t* row_mask, orlhf_stream_t stream) {
+                                      const uint8_t* row_mask, void* workspace, int64_t workspace_bytes,
+                                      int32_t* tickets, orlhf_stream_t stream) {
   const int bad = check_top("top_logprobs_fwd", dtype, n_rows, vocab, row_stride, temperature, k);
   if (bad != ORLHF_OK) return bad;
   if (n_rows == 0) return ORLHF_OK;  // nothing to launch; empty arrays may well be NULL
@@ -778,8 +665,14 @@ extern "C" int orlhf_top_logprobs_fwd(const void* logits, int dtype, int64_t n_r
   ORLHF_CHECK_ARG(((uintptr_t)logits & (dtype == ORLHF_F32 ? 3u : 1u)) == 0,
                   "top_logprobs_fwd: logits not aligned to the element size");
   const int64_t esize = dtype == ORLHF_F32 ? 4 : 2;
+  const int64_t need = orlhf_top_logprobs_workspace_bytes(dtype, n_rows, vocab, k);
+  ORLHF_CHECK_ARG(need == 0 || (workspace != nullptr && workspace_bytes >= need && ((uintptr_t)workspace & 7u) == 0),
+                  "top_logprobs_fwd: this shape needs %lld bytes of 8-byte aligned workspace, got %lld", (long long)need,
+                  (long long)workspace_bytes);
+  ORLHF_CHECK_ARG(((uintptr_t)tickets & 3u) == 0, "top_logprobs_fwd: tickets not 4-byte aligned");
   const TopArgs a = {(const char*)logits, n_rows, vocab, row_stride * esize, labels, temperature, (int)k, logprob,
-                     entropy, top_logprob, row_stats, top_ids, row_mask, 0};
+                     entropy, top_logprob, row_stats, top_ids, row_mask, 0, list_split(n_rows, vocab, (int)esize),
+                     (uint64_t*)workspace, tickets};
   hipStream_t s = (hipStream_t)stream;
   switch (dtype) {
     case ORLHF_F32: return launch_top_fwd<ORLHF_F32>(a, s);
@@ -811,7 +704,7 @@ extern "C" int orlhf_top_logprobs_bwd(const void* logits, void* grad_logits, int
                           (((row_stride - grad_row_stride) * esize) & 15) == 0;
   const TopBwdArgs a = {(const char*)logits, (char*)grad_logits, n_rows, vocab, row_stride * esize, grad_row_stride * esize,
                         labels, top_ids, temperature, (int)k, g_logprob, g_entropy, g_top_logprob, row_stats, row_mask,
-                        same_phase ? 0 : 1};
+                        same_phase ? 0 : 1, list_split(n_rows, vocab, (int)esize)};
   hipStream_t s = (hipStream_t)stream;
   switch (dtype) {
     case ORLHF_F32: return launch_top_bwd<ORLHF_F32>(a, s);

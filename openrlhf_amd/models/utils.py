@@ -52,13 +52,14 @@ _TICKETS = {}  # (device index, stream handle) -> int32 tickets, all zero whenev
 def _row_tickets(dev, n_rows):
     """The tickets of the few-row forward: zero on entry, put back to zero by the kernel itself, so one
     array per (device, stream) serves every call (calls on one stream do not overlap). Allocated and
-    zeroed outside any graph capture: the few-row launch is at most 255 rows, so 256 always do."""
+    zeroed outside any graph capture and never replaced (a captured graph may hold its address): the
+    launches that cut rows have at most 511 of them, so 512 always do."""
     key = (dev.index if dev.index is not None else torch.cuda.current_device(), stream_of(dev))
     t = _TICKETS.get(key)
     if t is None or t.numel() < n_rows:
         if torch.cuda.is_current_stream_capturing():
             return None  # first use of this stream is under capture: the two-launch form needs no state
-        t = _TICKETS[key] = torch.zeros(max(256, n_rows), dtype=torch.int32, device=dev)
+        t = _TICKETS[key] = torch.zeros(max(512, n_rows), dtype=torch.int32, device=dev)
     return t
 
 
@@ -221,7 +222,19 @@ def _mask_rows(row_mask, batch_shape):
         return None
     if row_mask.shape != batch_shape:
         raise ValueError(f"row_mask shape {tuple(row_mask.shape)} != logits batch shape {tuple(batch_shape)}")
-    return (row_mask != 0).reshape(-1).to(torch.uint8).contiguous()
+    if row_mask.dtype == torch.bool:
+        return row_mask.reshape(-1).contiguous().view(torch.uint8)
+    return (row_mask != 0).reshape(-1).view(torch.uint8)
+
+
+def _list_workspace(ws_bytes, n_rows, dev):
+    """(workspace, tickets) of a launch that cuts its rows into segments, (None, None) of one that does
+    not. No tickets under graph capture: two graphs captured on one stream may be replayed at the same
+    time on others, and would share the array; the two-launch form keeps no state."""
+    if ws_bytes == 0:
+        return None, None
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+    return ws, None if torch.cuda.is_current_stream_capturing() else _row_tickets(dev, n_rows)
 
 
 def _f32_rows(t, shape, name):
@@ -257,8 +270,11 @@ class _TopLogprobs(torch.autograd.Function):
         ids = torch.empty((n_rows, k), device=dev, dtype=torch.int64)
         stats = torch.empty((n_rows, 4), **opts) if needs_grad else None
         with _lib.on_device(dev):
+            ws_bytes = _lib.load().orlhf_top_logprobs_workspace_bytes(code, n_rows, vocab, k)
+            ws, tickets = _list_workspace(ws_bytes, n_rows, dev)
             call("orlhf_top_logprobs_fwd", ptr(rows), code, n_rows, vocab, row_stride, ptr(lab), float(temperature), k,
-                 ptr(logprob), ptr(entropy), ptr(top), ptr(ids), ptr(stats), ptr(rmask), stream_of(dev))
+                 ptr(logprob), ptr(entropy), ptr(top), ptr(ids), ptr(stats), ptr(rmask), ptr(ws), ws_bytes, ptr(tickets),
+                 stream_of(dev))
         ctx.temperature, ctx.k = float(temperature), k
         ctx.inplace = bool(inplace_backward) and aliases
         ctx.row_stride = row_stride

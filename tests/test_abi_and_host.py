@@ -349,8 +349,8 @@ def test_top_logprobs_entries_refuse_bad_arguments(lib):
     def err():
         return lib.orlhf_last_error().decode()
 
-    fwd = lambda n=2, v=64, stride=64, t=1.0, k=4, x=8, dt=1, top=8: lib.orlhf_top_logprobs_fwd(  # noqa: E731
-        x, dt, n, v, stride, None, t, k, None, None, top, 8, None, None, None)
+    fwd = lambda n=2, v=64, stride=64, t=1.0, k=4, x=8, dt=1, top=8, ws=None, nb=0, tick=None: lib.orlhf_top_logprobs_fwd(  # noqa: E731
+        x, dt, n, v, stride, None, t, k, None, None, top, 8, None, None, ws, nb, tick, None)
     assert fwd(k=0) == -1 and "k=0" in err()
     assert fwd(k=129, v=1000, stride=1000) == -1 and "k=129" in err()
     assert fwd(k=65) == -1 and "exceed vocab" in err()
@@ -362,6 +362,12 @@ def test_top_logprobs_entries_refuse_bad_arguments(lib):
     assert fwd(x=9) == -1 and "aligned" in err()
     assert fwd(top=None) == -1 and "NULL" in err()
     assert fwd(n=0, x=None) == 0
+    # few long rows are cut into segments and need a workspace
+    need = lib.orlhf_top_logprobs_workspace_bytes(1, 2, 151936, 4)
+    assert need > 0 and need % 8 == 0 and lib.orlhf_top_logprobs_workspace_bytes(1, 4096, 151936, 4) == 0
+    for bad in (dict(), dict(ws=8, nb=need - 1), dict(ws=4, nb=need)):
+        assert fwd(v=151936, stride=151936, **bad) == -1 and "workspace" in err()
+    assert fwd(tick=2) == -1 and "tickets" in err()
     bwd = lambda glp=None, gh=None, gtop=None, ids=None, gs=64: lib.orlhf_top_logprobs_bwd(  # noqa: E731
         8, 8, 1, 2, 64, 64, gs, None, 1.0, 4, ids, glp, gh, gtop, 8, None, None)
     assert bwd() == -1 and "every upstream" in err()

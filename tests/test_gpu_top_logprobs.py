@@ -69,6 +69,10 @@ def _check_forward(view, labels, k, temperature, out, row_mask=None):
     (260, 32000, 8, "fp32", 1.0, 0, 0),
     (7, 50257, 128, "bf16", 0.6, 2, 1),
     (3, 151936, 1, "bf16", 1.0, 0, 0),
+    (1, 151937, 128, "bf16", 1.0, 0, 5),
+    (511, 20011, 30, "fp32", 0.9, 0, 0),
+    (512, 20011, 30, "bf16", 1.0, 0, 0),
+    (2, 524309, 128, "fp32", 1.0, 0, 1),
     (65, 151936, 20, "bf16", 1.0, 0, 0),
     (2, 262144, 100, "fp16", 0.6, 0, 0),
     (270, 70001, 5, "bf16", 1.0, 0, 0),
@@ -248,14 +252,15 @@ def test_gradients_of_masked_vocabularies(cuda, dtype):
     _check_grad(x[:1, :20].cuda(), grad[:1, :20], labels[:1], out[3].cpu()[:1], gs[0][:1], gs[1][:1], gs[2][:1], 1.0, [0])
 
 
-def test_masked_rows_and_labels_outside(cuda):
+@pytest.mark.parametrize("vocab", [4099, 40009])
+def test_masked_rows_and_labels_outside(cuda, vocab):
     from openrlhf_amd.models.utils import top_logprobs_from_logits
 
-    view, labels, g = _logits(40, 4099, "bf16", 21)
+    view, labels, g = _logits(40, vocab, "bf16", 21)
     view = view.detach().requires_grad_(True)
     mask = torch.rand(40, generator=g) < 0.5
     mask[0], mask[1], mask[2] = True, True, False
-    labels[0], labels[1] = -100, 4099
+    labels[0], labels[1] = -100, vocab
     lp, ent, top, ids = top_logprobs_from_logits(view, labels.cuda().int(), 6, row_mask=mask.cuda())
     assert lp[0].item() == 0.0 and math.isnan(lp[1].item())
     inside = labels.clone()
@@ -287,6 +292,44 @@ def test_shapes_strides_and_absent_outputs(cuda):
     assert ((top2 - top).abs() <= 64 * U * (1 + top.abs())).all()
     empty = top_logprobs_from_logits(x[:0], labels[:0], 4)
     assert [tuple(t.shape) for t in empty] == [(0, 3), (0, 3), (0, 3, 4), (0, 3, 4)]
+
+
+@pytest.mark.parametrize("rows,vocab,k", [(1, 151936, 20), (7, 151936, 128), (300, 50257, 20), (64, 262144, 64)])
+def test_cut_rows_merged_in_one_launch_or_two_give_the_same_bits(cuda, rows, vocab, k):
+    """The records of a cut row are merged by the workgroup that finishes it (tickets) or by a second
+    launch; repeated calls over one ticket array, with masked rows, a row of equal logits (more
+    candidates than fit) and one with a NaN among them."""
+    from openrlhf_amd import _lib
+
+    view, labels, g = _logits(rows, vocab, "bf16", rows + k)
+    if rows > 3:
+        view[0] = 0.25
+        view[1, 77] = math.nan
+        view[2, : vocab - 9] = -math.inf
+    lab = labels.cuda()
+    mask = torch.ones(rows, dtype=torch.uint8, device="cuda")
+    mask[rows // 2 : rows // 2 + rows // 5] = 0
+    lib = _lib.load()
+    nbytes = lib.orlhf_top_logprobs_workspace_bytes(_lib.BF16, rows, vocab, k)
+    assert nbytes > 0
+    tickets = torch.zeros(rows, dtype=torch.int32, device="cuda")
+
+    def once(tick):
+        ws = torch.randint(0, 255, (nbytes,), dtype=torch.uint8, device="cuda")
+        lp, ent = torch.full((rows,), 7.0, device="cuda"), torch.full((rows,), 7.0, device="cuda")
+        top, stats = torch.full((rows, k), 7.0, device="cuda"), torch.full((rows, 4), 7.0, device="cuda")
+        ids = torch.full((rows, k), 7, device="cuda")
+        _lib.call("orlhf_top_logprobs_fwd", view.data_ptr(), _lib.BF16, rows, vocab, vocab, lab.data_ptr(), 0.8, k,
+                  lp.data_ptr(), ent.data_ptr(), top.data_ptr(), ids.data_ptr(), stats.data_ptr(), mask.data_ptr(),
+                  ws.data_ptr(), nbytes, None if tick is None else tick.data_ptr(), _lib.stream_of(view.device))
+        return [t.view(torch.int32) if t.dtype == torch.float32 else t for t in (lp, ent, top, ids, stats)]
+
+    want = once(None)
+    for _ in range(20):
+        got = once(tickets)
+        assert int(tickets.abs().sum()) == 0
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
 
 
 @pytest.mark.parametrize("rows", [2, 300])
