@@ -22,9 +22,14 @@ struct RowSoftmax {
   float centre, l2_t, l2_1, ex;  // the backward's statistics: softmax(x / T) = 2^((x - centre) cT - l2_t)
 };
 
+// Two accumulators per sum: the waves of six workgroups per CU hide the rest of the adders' latency, and
+// the registers of a third and fourth would cost one of the six.
+template <int MODE>
+using ListAcc = FastAcc<MODE, 2>;
+
 // Fast pass: per wave sums against its reference, folded over the workgroup.
 template <int MODE>
-__device__ __forceinline__ RowSums combine_fast(const FastAcc<MODE>& acc, float (*lds)[8]) {
+__device__ __forceinline__ RowSums combine_fast(const ListAcc<MODE>& acc, float (*lds)[8]) {
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
   float st, s, t;
   acc.fold(st, s, t);

@@ -35,7 +35,7 @@ struct Candidates {
 };
 
 // How many of the n candidates rank before each of this thread's (at threadIdx.x + i * kBlock). The
-// candidates are read eight at a time, all lanes the same: a broadcast.
+// candidates are read two by two, all lanes the same: a broadcast.
 typedef uint64_t u64x2 __attribute__((ext_vector_type(2)));
 template <int MINE>
 __device__ __forceinline__ void rank_candidates(const Candidates& c, int n, uint64_t (&mine)[MINE], int (&rank)[MINE]) {
@@ -50,13 +50,14 @@ __device__ __forceinline__ void rank_candidates(const Candidates& c, int n, uint
 #pragma unroll
     for (int i = 0; i < MINE; ++i) rank[i] += other > mine[i] ? 1 : 0;
   };
+  constexpr int kAhead = MINE == 1 ? 4 : 1;  // more of them in registers where the usual rows come by
   int j = 0;
-  for (; j + 8 <= n; j += 8) {
-    u64x2 two[4];
+  for (; j + 2 * kAhead <= n; j += 2 * kAhead) {
+    u64x2 two[kAhead];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) two[q] = *(const u64x2*)(c.key + j + 2 * q);
+    for (int q = 0; q < kAhead; ++q) two[q] = *(const u64x2*)(c.key + j + 2 * q);
 #pragma unroll
-    for (int q = 0; q < 4; ++q) count(two[q][0]), count(two[q][1]);
+    for (int q = 0; q < kAhead; ++q) count(two[q][0]), count(two[q][1]);
   }
   for (; j < n; ++j) count(c.key[j]);
 }
@@ -109,24 +110,18 @@ __device__ __forceinline__ void collect_row(const char* row, const RowGeom& g, u
   const char* body = row + g.head * E::kSize;
 #pragma unroll 1
   for (uint32_t v0 = 0; v0 < g.nvec; v0 += kBlock) {
-    const uint32_t v = v0 + tid;
-    uint64_t key[EPV];
+    const uint32_t v = v0 + tid, id = first + g.head + v * EPV;
     bool any = false;
-    float x[EPV];
-    if (v < g.nvec) E::unpack(*(const u32x4*)(body + v * 16u), x);
+    if (v < g.nvec) {
+      float x[EPV];
+      E::unpack(*(const u32x4*)(body + v * 16u), x);
 #pragma unroll
-    for (int j = 0; j < EPV; ++j) {
-      key[j] = v < g.nvec ? make_key(x[j], first + g.head + v * EPV + j) : 0ull;
-      any = any || key[j] > least;
+      for (int j = 0; j < EPV; ++j) any = any || make_key(x[j], id + j) > least;
     }
     if (__syncthreads_or(any)) {
 #pragma unroll 1
-      for (int j = 0; j < EPV; ++j) {  // not unrolled: the candidates' thinning is a large piece of code
-        uint64_t mine = 0;
-#pragma unroll
-        for (int i = 0; i < EPV; ++i) mine = i == j ? key[i] : mine;
-        push_round(c, mine, k, least);
-      }
+      for (int j = 0; j < EPV; ++j)  // rare rows: read once more rather than held in registers
+        push_round(c, v < g.nvec ? make_key(E::load1(body + v * 16u + j * E::kSize), id + j) : 0ull, k, least);
     }
   }
   const uint32_t nscalar = g.head + g.tail;
@@ -198,7 +193,7 @@ __device__ __forceinline__ float quad_maxima(const float (&m)[4]) {
 // asked for ahead by each workgroup at any time. The wave's exponent reference is the maximum of its
 // lanes' first blocks.
 template <int DT, int MODE>
-__device__ __forceinline__ float stream_row(const char* row, const RowGeom& g, float c_scaled, FastAcc<MODE>& acc,
+__device__ __forceinline__ float stream_row(const char* row, const RowGeom& g, float c_scaled, ListAcc<MODE>& acc,
                                             float* block_max, int shift) {
   using E = Elt<DT>;
   constexpr int EPV = E::kPerVec;
@@ -457,7 +452,7 @@ __global__ __launch_bounds__(kBlock) void top_logprobs_fwd_kernel(TopArgs a) {
     const int64_t at = label - (int64_t)seg.first;
     if (at >= 0 && at < seg.len) x_label = E::load1(row + at * E::kSize);
   }
-  FastAcc<MODE> acc;
+  ListAcc<MODE> acc;
   const float thread_max = stream_row<DT, MODE>(row, g, (float)(1.4426950408889634 / a.temperature), acc, block_max, a.shift);
   sh.best[tid] = ordered_bits(thread_max);
   const RowSums sums = combine_fast<MODE>(acc, sh.lds);  // its barriers also publish the maxima

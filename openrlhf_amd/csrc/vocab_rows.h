@@ -249,17 +249,17 @@ __device__ __forceinline__ void traverse_row(const char* row, char* out_row, con
 constexpr int kAcc = 4;  // independent accumulators per lane
 
 // Fast path: exponent = x*c - M with a wave-uniform reference M (no running maximum).
-template <int MODE>
+template <int MODE, int ACC = kAcc>
 struct FastAcc {
   float cT, negMT, c1, negM1;
-  float sT[kAcc], s1[kAcc], t1[kAcc];
+  float sT[ACC], s1[ACC], t1[ACC];
   __device__ __forceinline__ void init(float m_ref, float c_scaled, float c_plain) {
     cT = c_scaled;
     c1 = c_plain;
     negMT = -(m_ref * c_scaled);
     negM1 = -(m_ref * c_plain);
 #pragma unroll
-    for (int k = 0; k < kAcc; ++k) sT[k] = s1[k] = t1[k] = 0.0f;
+    for (int k = 0; k < ACC; ++k) sT[k] = s1[k] = t1[k] = 0.0f;
   }
   __device__ __forceinline__ void elem(float x, int k) {
     if (ModeTraits<MODE>::kScaledSet) sT[k] += fast_exp2(fmaf(x, cT, negMT));
@@ -272,13 +272,20 @@ struct FastAcc {
   template <int N>
   __device__ __forceinline__ void vec(float (&x)[N], uint32_t) {
 #pragma unroll
-    for (int j = 0; j < N; ++j) elem(x[j], j % kAcc);
+    for (int j = 0; j < N; ++j) elem(x[j], j % ACC);
   }
   __device__ __forceinline__ void one(float& x, uint32_t) { elem(x, 0); }
   __device__ __forceinline__ void fold(float& st, float& s, float& t) const {
-    st = (sT[0] + sT[1]) + (sT[2] + sT[3]);
-    s = (s1[0] + s1[1]) + (s1[2] + s1[3]);
-    t = (t1[0] + t1[1]) + (t1[2] + t1[3]);
+    static_assert(ACC == 2 || ACC == 4, "fold adds pairs");
+    if (ACC == 4) {
+      st = (sT[0] + sT[1]) + (sT[ACC - 2] + sT[ACC - 1]);
+      s = (s1[0] + s1[1]) + (s1[ACC - 2] + s1[ACC - 1]);
+      t = (t1[0] + t1[1]) + (t1[ACC - 2] + t1[ACC - 1]);
+    } else {
+      st = sT[0] + sT[1];
+      s = s1[0] + s1[1];
+      t = t1[0] + t1[1];
+    }
   }
 };
 
