@@ -25,7 +25,17 @@ struct RowSoftmax {
 // Two accumulators per sum: the waves of six workgroups per CU hide the rest of the adders' latency, and
 // the registers of a third and fourth would cost one of the six.
 template <int MODE>
-using ListAcc = FastAcc<MODE, 2>;
+struct ListAcc : FastAcc<MODE, 2> {
+  // The sums so far are taken as used here, by no instruction: the compiler otherwise moves the
+  // exponentials of several vectors behind the next branch and keeps all their elements until then.
+  __device__ __forceinline__ void settle() {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      if (ModeTraits<MODE>::kScaledSet) asm volatile("" : "+v"(this->sT[k]));
+      if (ModeTraits<MODE>::kPlainSet) asm volatile("" : "+v"(this->s1[k]), "+v"(this->t1[k]));
+    }
+  }
+};
 
 // Fast pass: per wave sums against its reference, folded over the workgroup.
 template <int MODE>

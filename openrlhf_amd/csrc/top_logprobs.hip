@@ -170,7 +170,7 @@ __device__ __forceinline__ void write_skipped_row(const TopArgs& a, int64_t row_
 // (expected -256 ln(1 - k/256): 20 for k = 20, 177 for k = 128), so only the blocks that reach it are
 // read again, about 64 k bytes per row, and their elements that reach it become candidates. (Blocks of
 // one lane's four vectors need no exchange but lie 4 KiB apart, and reading them again fetched an
-// eighth of the row: 221 against 197 us at 4096 x 151936 bf16, k = 64.) A row that has more candidates
+// eighth of the row: 221 against 208 us at 4096 x 151936 bf16, k = 64.) A row that has more candidates
 // than fit (many equal logits), or a NaN, goes through collect_row instead.
 constexpr int kMaxBlocks = 32;
 constexpr uint32_t kBlockVecs = 4;  // vectors in a block, and a thread's loads per step
@@ -189,9 +189,10 @@ __device__ __forceinline__ float quad_maxima(const float (&m)[4]) {
   return with_neighbour(high ? hi : lo, high ? lo : hi, kSwap2);
 }
 
-// The loads of the next block are in flight while one is worked on: two blocks of registers, 16 KiB
-// asked for ahead by each workgroup at any time. The wave's exponent reference is the maximum of its
-// lanes' first blocks.
+// The loads of the next step are in flight while one is worked on: two steps of registers, 16 KiB
+// asked for ahead by each workgroup at any time. The vectors past the last whole step come first, so
+// that the loop has no predicated step (after one the compiler waits for every load before it issues
+// the next). The wave's exponent reference is the maximum of its lanes' first vectors.
 template <int DT, int MODE>
 __device__ __forceinline__ float stream_row(const char* row, const RowGeom& g, float c_scaled, ListAcc<MODE>& acc,
                                             float* block_max, int shift) {
@@ -201,62 +202,79 @@ __device__ __forceinline__ float stream_row(const char* row, const RowGeom& g, f
   const uint32_t tid = threadIdx.x;
   const char* body = row + g.head * E::kSize;
   float thread_max = -INFINITY;
-  const uint32_t parts = (g.nvec + kStep - 1) / kStep;
-  auto load = [&](u32x4 (&raw)[kBlockVecs], uint32_t part) {  // past the end: the last vector again, not used
+  const uint32_t whole = g.nvec / kStep, rest = g.nvec - whole * kStep;
+  auto load = [&](u32x4 (&raw)[kBlockVecs], uint32_t step) {
+    const uint32_t at = step * (kStep * 16u) + tid * 16u;
 #pragma unroll
-    for (uint32_t u = 0; u < kBlockVecs; ++u) {
-      const uint32_t v = part * kStep + u * kBlock + tid;
-      raw[u] = load_vec(body + (v < g.nvec ? v : g.nvec - 1) * 16u);
-    }
+    for (uint32_t u = 0; u < kBlockVecs; ++u) raw[u] = load_vec(body + (at + u * (kBlock * 16u)));
+    __builtin_amdgcn_sched_barrier(0);  // all of them issued before the work on the step at hand
   };
-  auto consume = [&](const u32x4 (&raw)[kBlockVecs], uint32_t part) {
-    float m[kBlockVecs] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-    const uint32_t v0 = part * kStep + tid;
-    auto take = [&](uint32_t u) {
-      float x[EPV];
-      E::unpack(raw[u], x);
-#pragma unroll
-      for (int j = 0; j < EPV; ++j) m[u] = fmaxf(m[u], x[j]);
-      acc.vec(x, 0);
-    };
-    if ((part + 1) * kStep <= g.nvec) {
-#pragma unroll
-      for (uint32_t u = 0; u < kBlockVecs; ++u) take(u);
-    } else {
-#pragma unroll
-      for (uint32_t u = 0; u < kBlockVecs; ++u)
-        if (v0 + u * kBlock < g.nvec) take(u);
-    }
+  auto note = [&](uint32_t step, const float (&m)[kBlockVecs]) {
     const float bm = quad_maxima(m);
-    float* slot = block_max + (part >> shift) * kBlock + tid;
-    *slot = (part & ((1u << shift) - 1u)) == 0u ? bm : fmaxf(*slot, bm);
+    float* slot = block_max + (step >> shift) * kBlock + tid;
+    // the remainder (step == whole) is noted first: it opens its slot, the others of the slot add to it
+    const bool opens = (step & ((1u << shift) - 1u)) == 0u && (shift == 0 || rest == 0u || (step >> shift) != (whole >> shift));
+    *slot = opens || step == whole ? bm : fmaxf(*slot, bm);
     thread_max = fmaxf(thread_max, bm);
   };
+  auto take = [&](const u32x4& raw, float& m) {
+    uint32_t w0 = raw[0], w1 = raw[1], w2 = raw[2], w3 = raw[3];
+    asm volatile("" : "+v"(w0), "+v"(w1), "+v"(w2), "+v"(w3));  // unpacked here, not ahead for several vectors
+    float x[EPV];
+    E::unpack(u32x4{w0, w1, w2, w3}, x);
+#pragma unroll
+    for (int j = 0; j < EPV; ++j) m = fmaxf(m, x[j]);
+    acc.vec(x, 0);
+    acc.settle();  // one vector's values at a time: registers decide how many rows a CU holds
+  };
+  auto consume = [&](const u32x4 (&raw)[kBlockVecs], uint32_t step) {
+    float m[kBlockVecs] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+    for (uint32_t u = 0; u < kBlockVecs; ++u) take(raw[u], m[u]);
+    note(step, m);
+  };
+  auto raise = [&](const u32x4& raw, float& m) {
+    float x[EPV];
+    E::unpack(raw, x);
+#pragma unroll
+    for (int j = 0; j < EPV; ++j) m = fmaxf(m, x[j]);
+  };
+
   u32x4 ping[kBlockVecs], pong[kBlockVecs];
-  if (parts > 0) load(ping, 0);
+#pragma unroll
+  for (uint32_t u = 0; u < kBlockVecs; ++u)
+    if (u * kBlock + tid < rest) pong[u] = load_vec(body + (whole * kStep + u * kBlock + tid) * 16u);
+  if (whole > 0) load(ping, 0);
   // head and tail of a row off the 16-byte grid: at most one element per thread
   const uint32_t nscalar = g.head + g.tail;
   float xs = -INFINITY;
   if (tid < nscalar) xs = E::load1(row + (tid < g.head ? tid : g.nvec * EPV + tid) * E::kSize);
   float m_ref = xs;
-  if (parts > 0) {
-#pragma unroll
-    for (uint32_t u = 0; u < kBlockVecs; ++u) {
-      float x[EPV];
-      E::unpack(ping[u], x);
-#pragma unroll
-      for (int j = 0; j < EPV; ++j) m_ref = fmaxf(m_ref, x[j]);
-    }
-  }
+  if (tid < rest) raise(pong[0], m_ref);
+  if (whole > 0) raise(ping[0], m_ref);
   acc.init(wave_max(m_ref), c_scaled, kLog2e);
   if (tid < nscalar) acc.one(xs, 0);
-  for (uint32_t part = 0; part < parts;) {
-    if (part + 1 < parts) load(pong, part + 1);
-    consume(ping, part);
-    if (++part >= parts) break;
-    if (part + 1 < parts) load(ping, part + 1);
-    consume(pong, part);
-    ++part;
+  if (rest > 0) {
+    float m[kBlockVecs] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+    for (uint32_t u = 0; u < kBlockVecs; ++u)
+      if (u * kBlock + tid < rest) take(pong[u], m[u]);
+    note(whole, m);
+  }
+  if (whole == 0) return thread_max;
+  uint32_t step = 0;
+  for (; step + 2 < whole; step += 2) {
+    load(pong, step + 1);
+    consume(ping, step);
+    load(ping, step + 2);
+    consume(pong, step + 1);
+  }
+  if (step + 1 < whole) {
+    load(pong, step + 1);
+    consume(ping, step);
+    consume(pong, step + 1);
+  } else {
+    consume(ping, step);
   }
   return thread_max;
 }
