@@ -58,6 +58,11 @@ enum orlhf_pair_loss {
   ORLHF_PAIR_LOGSIGMOID = 2,  /* PairWiseLoss: -logsigmoid(chosen - rejected [- margin])    */
   ORLHF_PAIR_LOGEXP = 3       /* LogExpLoss: log(1 + exp(rejected - chosen))                */
 };
+enum orlhf_distill {
+  ORLHF_DISTILL_FORWARD_TAIL = 0, /* KL(teacher || student) over the listed tokens and one outcome for the rest */
+  ORLHF_DISTILL_FORWARD = 1,      /* KL(teacher renormalised over the list || student's full softmax)           */
+  ORLHF_DISTILL_REVERSE_TAIL = 2  /* KL(student || teacher) over the listed tokens and one outcome for the rest */
+};
 enum orlhf_group_estimator {
   ORLHF_GROUP_IDENTITY = 0, /* gae, reinforce: rewards unchanged                                 */
   ORLHF_GROUP_RLOO = 1,     /* r - (sum - r)/(n-1)                                               */
@@ -193,6 +198,43 @@ int orlhf_top_logprobs_bwd(const void* logits, void* grad_logits, int dtype, int
                            const int64_t* top_ids, const float* g_logprob, const float* g_entropy,
                            const float* g_top_logprob, const float* row_stats,
                            const uint8_t* row_mask, orlhf_stream_t stream);
+
+/*
+ * Distillation from a teacher known by its most likely tokens: KL divergence per row between the
+ * teacher's list (teacher_ids int64 [n_rows, k], teacher_logprob float [n_rows, k]) and the student's
+ * q = softmax(logits / temperature). With p = exp(teacher_logprob), P = sum p, t = 1 - P and
+ * s = 1 - (q's mass on the list, but summed directly):
+ *   FORWARD_TAIL  sum p (log p - log q) + t (log t - log s)     (t >= 0)
+ *   FORWARD       sum w (log w - log q), w = softmax over the list of teacher_logprob / teacher_temperature
+ *   REVERSE_TAIL  sum q (log q - log p) + s (log s - log t)     (t >= 2^-24)
+ * s is taken to be at least 2^-126. teacher_temperature is 1 for the kinds with a tail; for FORWARD the
+ * values may be logits. 1 <= k <= 128. An entry with a negative id or a value of -inf is absent; an id
+ * that comes twice counts once, with the sum of its probabilities; an id past the vocabulary makes the
+ * row's loss NaN and gets no gradient; a row without entries has loss 0 and gradient 0. Rows with
+ * row_mask 0 are not read: loss 0. vocab <= 520192 (ORLHF_ERR_UNSUPPORTED beyond).
+ *   loss       float [n_rows]
+ *   row_stats  float [n_rows, 4], list_grad float [n_rows, k], list_at int32 [n_rows, k]: what the
+ *              backward needs, all three or none (NULL)
+ * workspace and tickets as in orlhf_top_logprobs_fwd. No reference counterpart in this version.
+ */
+int64_t orlhf_distill_kl_workspace_bytes(int dtype, int64_t n_rows, int64_t vocab);
+int orlhf_distill_kl_fwd(const void* logits, int dtype, int64_t n_rows, int64_t vocab,
+                         int64_t row_stride, const int64_t* teacher_ids, const float* teacher_logprob,
+                         int64_t k, double temperature, double teacher_temperature, int kind,
+                         float* loss, float* row_stats, float* list_grad, int32_t* list_at,
+                         const uint8_t* row_mask, void* workspace, int64_t workspace_bytes,
+                         int32_t* tickets, orlhf_stream_t stream);
+
+/*
+ * Its backward: grad[i,j] = g_loss[i] * d loss[i] / d logits[i,j], in the logits dtype; `grad_logits`
+ * may alias `logits` (same row stride). Rows with g_loss 0 or row_mask 0 are written as zeros without
+ * being read.
+ */
+int orlhf_distill_kl_bwd(const void* logits, void* grad_logits, int dtype, int64_t n_rows,
+                         int64_t vocab, int64_t row_stride, int64_t grad_row_stride, int64_t k,
+                         double temperature, const float* g_loss, const float* row_stats,
+                         const float* list_grad, const int32_t* list_at, const uint8_t* row_mask,
+                         orlhf_stream_t stream);
 
 /*
  * Forward and backward in ONE pass for callers that know the upstream weights when the forward

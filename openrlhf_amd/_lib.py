@@ -20,6 +20,7 @@ AGG_TOKEN_MEAN, AGG_SEQ_MEAN, AGG_ROW_MEAN, AGG_SEQ_MEAN_TOKEN_SUM = 0, 1, 2, 3
 POLICY_PPO, POLICY_GSPO = 0, 1
 IS_NONE, IS_TIS, IS_ICEPOP, IS_SEQ_MASK_TIS = 0, 1, 2, 3
 GROUP_IDENTITY, GROUP_RLOO, GROUP_BASELINE, GROUP_NORM = 0, 1, 2, 3
+DISTILL_FORWARD_TAIL, DISTILL_FORWARD, DISTILL_REVERSE_TAIL = 0, 1, 2
 PAIR_DPO_SIGMOID, PAIR_DPO_IPO, PAIR_LOGSIGMOID, PAIR_LOGEXP = 0, 1, 2, 3
 
 ABI_VERSION = 23
@@ -86,6 +87,10 @@ SIGNATURES = {
     "orlhf_top_logprobs_workspace_bytes": (I64, [c_int, I64, I64, I64]),
     "orlhf_top_logprobs_fwd": (c_int, [P, c_int, I64, I64, I64, P, c_double, I64, P, P, P, P, P, P, P, I64, P, P]),
     "orlhf_top_logprobs_bwd": (c_int, [P, P, c_int, I64, I64, I64, I64, P, c_double, I64, P, P, P, P, P, P, P]),
+    "orlhf_distill_kl_workspace_bytes": (I64, [c_int, I64, I64]),
+    "orlhf_distill_kl_fwd": (c_int, [P, c_int, I64, I64, I64, P, P, I64, c_double, c_double, c_int, P, P, P, P, P, P, I64, P,
+                                     P]),
+    "orlhf_distill_kl_bwd": (c_int, [P, P, c_int, I64, I64, I64, I64, I64, c_double, P, P, P, P, P, P]),
     "orlhf_lmhead_workspace_bytes": (I64, [I64, I64, I64, I64, c_int]),
     "orlhf_lmhead_logprob_entropy_fwd": (c_int, [P, P, c_int, I64, I64, I64, I64, I64, P, c_double, P, P, P, P, I64, I64,
                                                  P, I64, P]),

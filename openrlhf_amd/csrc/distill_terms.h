@@ -1,0 +1,228 @@
+// KL divergence of one vocabulary row between a teacher known by a list of tokens and the student's full
+// softmax q of x / T: the list, the student's sum without it, and the loss with its derivatives.
+//
+//   kind            loss                                                     dL/dz_listed      dL/dz_other
+//   forward, tail   sum p (log p - log q) + t (log t - log s)                (P+t) q - p       (P+t - t/s) q
+//   forward         sum w (log w - log q),  w = p / P                        q - w             q
+//   reverse, tail   sum q (log q - log p) + s (log s - log t)                q (r - L)         q (log s/t - L)
+//
+// with P = sum p, t = 1 - P (at least 0; in the reverse form at least 2^-24, what a sum of fp32
+// probabilities resolves), s the student's mass outside the list, r = log q - log p, z = x / T. The
+// gradient of every other element is one number times q: the backward is a softmax pass and a patch of
+// the listed elements. s is summed by itself, never as 1 - sum q: for a student that is sure of the listed
+// tokens that difference would be rounding noise, and log s and t / s with it.
+#pragma once
+#include "list_rows.h"
+
+namespace orlhf {
+
+constexpr int kMaxList = 128;                 // two entries per lane of one wave
+constexpr int64_t kMaxDistillVocab = 520192;  // a bit per element in 64 KiB of LDS, less the static part
+constexpr double kTinyTail = 5.9604644775390625e-08;  // 2^-24
+constexpr double kLogTinyRest = -87.33654475055310898657;  // log 2^-126: the student's tail mass is taken to be at least that
+
+// Teacher's list of one row and the student's logits there, held by one wave: entry lane + 64 i. An entry
+// with a negative id or a log-prob of -inf is absent, one past the vocabulary is absent and makes the
+// loss NaN, an id that comes twice counts once with the sum of its probabilities.
+struct ListEntries {
+  int id[2];     // -1: absent
+  float x[2];    // the student's logit
+  double lp[2];  // the teacher's log-prob
+  bool bad;
+};
+
+struct ListSource {
+  const int64_t* ids;
+  const float* teacher;
+  int k;
+  double inv_teacher_t;
+};
+
+template <int DT>
+__device__ __forceinline__ ListEntries load_list(const ListSource& src, int64_t row_i, const char* row, int64_t vocab) {
+  using E = Elt<DT>;
+  const int lane = threadIdx.x & (kWave - 1);
+  ListEntries e;
+  e.bad = false;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int at = lane + i * kWave;
+    const int64_t id = at < src.k ? src.ids[row_i * src.k + at] : -1;
+    const float v = at < src.k ? src.teacher[row_i * src.k + at] : -INFINITY;
+    const bool given = id >= 0 && v != -INFINITY;
+    e.bad = e.bad || (given && id >= vocab);
+    e.id[i] = given && id < vocab ? (int)id : -1;
+    e.lp[i] = (double)v * src.inv_teacher_t;
+    e.x[i] = e.id[i] >= 0 ? E::load1(row + (int64_t)e.id[i] * E::kSize) : 0.0f;
+  }
+  e.bad = __ballot(e.bad) != 0ull;
+  bool again[2] = {false, false};  // the id stands earlier in the list
+#pragma unroll 1
+  for (int j = 0; j < src.k - 1; ++j) {
+    const int other = j < kWave ? __builtin_amdgcn_readlane(e.id[0], j) : __builtin_amdgcn_readlane(e.id[1], j - kWave);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) again[i] = again[i] || (e.id[i] == other && other >= 0 && lane + i * kWave > j);
+  }
+  if (__ballot(again[0] || again[1]) != 0ull) {  // rare: add the later ones to the first
+    double sum[2] = {exp(e.lp[0]), exp(e.lp[1])};
+#pragma unroll 1
+    for (int j = 1; j < src.k; ++j) {
+      const bool second = j >= kWave;
+      const int other = __shfl(second ? e.id[1] : e.id[0], j & (kWave - 1), kWave);
+      const double lp = __shfl(second ? e.lp[1] : e.lp[0], j & (kWave - 1), kWave);
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        if (other >= 0 && e.id[i] == other && lane + i * kWave < j) sum[i] += exp(lp);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const double joint = log(sum[i]);
+      if (e.id[i] >= 0 && joint > e.lp[i]) e.lp[i] = joint;
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (again[i]) e.id[i] = -1;
+  }
+  return e;
+}
+
+// One bit per element of a row (or segment), set for the listed ones, in the order of the body's
+// elements: a vector of 8 elements is a byte, one of 4 half a byte. The scalars at the row's ends have
+// bits of their own behind it.
+template <int DT>
+struct ListMap {
+  static constexpr int EPV = Elt<DT>::kPerVec;
+  uint32_t* words;
+  uint32_t* ends;  // one word
+  static __host__ __device__ int64_t bytes(int64_t len) { return ((len + 127) / 128) * 16; }
+  __device__ __forceinline__ void clear(const RowGeom& g, int threads) const {
+    const uint32_t n16 = (g.nvec * EPV + 127u) / 128u;
+    for (uint32_t i = threadIdx.x; i < n16; i += threads) ((u32x4*)words)[i] = u32x4{0u, 0u, 0u, 0u};
+    if (threadIdx.x == 0) *ends = 0u;
+  }
+  __device__ __forceinline__ void set(const RowGeom& g, int64_t e, int64_t len) const {
+    if (e < 0 || e >= len) return;
+    const uint32_t i = (uint32_t)e, body = g.nvec * EPV;
+    if (i < g.head) {
+      atomicOr(ends, 1u << i);
+    } else if (i - g.head >= body) {
+      atomicOr(ends, 1u << (i - body));
+    } else {
+      atomicOr(words + (i - g.head) / 32u, 1u << ((i - g.head) % 32u));
+    }
+  }
+  __device__ __forceinline__ uint32_t vec(uint32_t v) const {
+    const uint8_t* b = (const uint8_t*)words;
+    return EPV == 8 ? b[v] : (uint32_t)(b[v >> 1] >> ((v & 1u) * 4u)) & 0xfu;
+  }
+  __device__ __forceinline__ bool scalar(uint32_t s) const { return (*ends >> s & 1u) != 0u; }
+};
+
+// Takes the listed elements out of the sums: their weight becomes that of -inf.
+template <int DT>
+struct WithoutListed {
+  ListMap<DT> map;
+  template <int N>
+  __device__ __forceinline__ void vec(float (&x)[N], uint32_t v) const {
+    const uint32_t bits = map.vec(v);
+    if (bits != 0u) {
+#pragma unroll
+      for (int j = 0; j < N; ++j) x[j] = (bits >> j & 1u) != 0u ? -INFINITY : x[j];
+    }
+  }
+  __device__ __forceinline__ void one(float& x, uint32_t s) const {
+    if (map.scalar(s)) x = -INFINITY;
+  }
+};
+
+__device__ __forceinline__ double wave_max(double v) {
+#pragma unroll
+  for (int o = kWave / 2; o > 0; o >>= 1) {
+    const double other = __shfl_xor(v, o, kWave);
+    v = other > v ? other : v;
+  }
+  return v;
+}
+
+struct ListTerms {
+  double loss, other;  // the loss and dL/dz / q of an element that is not listed
+  double grad[2];      // dL/dz of this lane's entries (0 where absent)
+  float centre, l2;    // q = 2^((x - centre) cT - l2)
+};
+
+// One wave. `sum`: the student's softmax sum, without the listed elements for the kinds with a tail, of
+// the whole row for the other. All of it in fp64: a few hundred operations of one wave per row.
+__device__ __forceinline__ ListTerms list_terms(const ListEntries& e, const RowTotals& sum, int kind, double temperature,
+                                                int64_t vocab) {
+  const bool tail = kind != ORLHF_DISTILL_FORWARD;
+  ListTerms r;
+  double z[2], p[2], lq[2], q[2];
+  int n_on = 0;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const bool on = e.id[i] >= 0;
+    n_on += __popcll(__ballot(on));
+    z[i] = on ? (double)e.x[i] / temperature : -INFINITY;
+    p[i] = on ? exp(e.lp[i]) : 0.0;
+  }
+  const double mass = wave_sum(p[0] + p[1]);
+  const bool some = sum.sT > 0.0 || sum.sT != sum.sT;  // anything of weight outside the list
+  double base = some ? sum.base_t : -INFINITY, total = sum.sT;
+  if (tail) {
+    const double top = wave_max(z[0] > z[1] ? z[0] : z[1]);
+    if (top > base) base = top;
+    double e01 = 0.0;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) e01 += e.id[i] >= 0 ? exp(z[i] - base) : 0.0;
+    total = (some ? sum.sT * exp(sum.base_t - base) : 0.0) + wave_sum(e01);
+  }
+  const double log_total = sum.nan ? (double)NAN : log(total);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    lq[i] = (z[i] - base) - log_total;
+    q[i] = e.id[i] >= 0 ? exp(lq[i]) : 0.0;
+  }
+  double log_s = some ? (sum.base_t - base) + log(sum.sT) - log_total : -INFINITY;
+  if (log_s < kLogTinyRest) log_s = kLogTinyRest;
+  const bool has_rest = n_on < vocab;
+  double part[2] = {0.0, 0.0};
+  if (kind == ORLHF_DISTILL_REVERSE_TAIL) {
+    const double t = fmax(1.0 - mass, kTinyTail), log_t = log(t), s = exp(log_s);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) part[i] = e.id[i] >= 0 && q[i] != 0.0 ? q[i] * (lq[i] - e.lp[i]) : 0.0;
+    r.loss = wave_sum(part[0] + part[1]) + (has_rest ? s * (log_s - log_t) : 0.0);
+    r.other = (log_s - log_t) - r.loss;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) r.grad[i] = part[i] - q[i] * r.loss;
+  } else {
+    const double log_mass = tail ? 0.0 : log(mass), scale = tail ? 1.0 : 1.0 / mass;
+    const double t = tail && has_rest ? fmax(1.0 - mass, 0.0) : 0.0;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      p[i] *= scale;
+      part[i] = p[i] != 0.0 ? p[i] * (e.lp[i] - log_mass - lq[i]) : 0.0;
+    }
+    r.loss = wave_sum(part[0] + part[1]) + (t > 0.0 ? t * (log(t) - log_s) : 0.0);
+    const double all = tail ? mass + t : 1.0;
+    r.other = all - (t > 0.0 ? t * exp(-log_s) : 0.0);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) r.grad[i] = e.id[i] >= 0 ? all * q[i] - p[i] : 0.0;
+  }
+  const double at = base * temperature;
+  r.centre = (float)at;
+  r.l2 = (float)((log_total + (at - (double)r.centre) / temperature) * 1.4426950408889634);
+  if (n_on == 0) {  // nothing to learn from: no loss, no gradient
+    r.loss = r.other = 0.0;
+    r.centre = r.l2 = 0.0f;
+  }
+  if (e.bad) r.loss = NAN;
+  return r;
+}
+
+// Coefficient of the softmax weight in an element's gradient. A weight that is 0 has to stay 0.
+__device__ __forceinline__ float grad_coef(double upstream, double other, double temperature) {
+  const double a = upstream * other / temperature;
+  return (float)(a > 3.0e38 ? 3.0e38 : (a < -3.0e38 ? -3.0e38 : a));
+}
+
+}  // namespace orlhf

@@ -73,6 +73,97 @@ __device__ __forceinline__ RowSums combine_fast(const ListAcc<MODE>& acc, float 
   return r;
 }
 
+// The fast pass of a workgroup over a row. The loads of the next step are in flight while one is worked
+// on: two steps of registers, 16 KiB asked for ahead by each workgroup at any time. The vectors past the
+// last whole step come first, so that the loop has no predicated step (after one the compiler waits for
+// every load before it issues the next). The wave's exponent reference is the maximum of its lanes' first
+// vectors. `watch` sees every vector before the sums do (and may change it), the scalars at a row's ends,
+// and, where it wants them, the maxima of each step; ready() is called once the first loads are on their way.
+constexpr uint32_t kStepVecs = 4;  // vectors per lane and step
+
+template <int DT, int MODE, typename W>
+__device__ __forceinline__ void stream_row(const char* row, const RowGeom& g, float c_scaled, ListAcc<MODE>& acc, W& watch) {
+  using E = Elt<DT>;
+  constexpr int EPV = E::kPerVec;
+  constexpr uint32_t kStep = kStepVecs * kBlock;
+  const uint32_t tid = threadIdx.x;
+  const char* body = row + g.head * E::kSize;
+  const uint32_t whole = g.nvec / kStep, rest = g.nvec - whole * kStep;
+  auto load = [&](u32x4 (&raw)[kStepVecs], uint32_t step) {
+    const uint32_t at = step * (kStep * 16u) + tid * 16u;
+#pragma unroll
+    for (uint32_t u = 0; u < kStepVecs; ++u) raw[u] = load_vec(body + (at + u * (kBlock * 16u)));
+    __builtin_amdgcn_sched_barrier(0);  // all of them issued before the work on the step at hand
+  };
+  auto unpacked = [&](const u32x4& raw, float (&x)[EPV], uint32_t v) {
+    uint32_t w0 = raw[0], w1 = raw[1], w2 = raw[2], w3 = raw[3];
+    asm volatile("" : "+v"(w0), "+v"(w1), "+v"(w2), "+v"(w3));  // unpacked here, not ahead for several vectors
+    E::unpack(u32x4{w0, w1, w2, w3}, x);
+    watch.vec(x, v);
+  };
+  auto take = [&](const u32x4& raw, float& m, uint32_t v) {
+    float x[EPV];
+    unpacked(raw, x, v);
+    if (W::kMaxima) {
+#pragma unroll
+      for (int j = 0; j < EPV; ++j) m = fmaxf(m, x[j]);
+    }
+    acc.vec(x, 0);
+    acc.settle();  // one vector's values at a time: registers decide how many rows a CU holds
+  };
+  auto consume = [&](const u32x4 (&raw)[kStepVecs], uint32_t step) {
+    float m[kStepVecs] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+    for (uint32_t u = 0; u < kStepVecs; ++u) take(raw[u], m[u], step * kStep + u * kBlock + tid);
+    if constexpr (W::kMaxima) watch.note(step, whole, rest, m);
+  };
+
+  u32x4 ping[kStepVecs], pong[kStepVecs];
+#pragma unroll
+  for (uint32_t u = 0; u < kStepVecs; ++u)
+    if (u * kBlock + tid < rest) pong[u] = load_vec(body + (whole * kStep + u * kBlock + tid) * 16u);
+  if (whole > 0) load(ping, 0);
+  // head and tail of a row off the 16-byte grid: at most one element per thread
+  const uint32_t nscalar = g.head + g.tail;
+  float xs = -INFINITY;
+  if (tid < nscalar) xs = E::load1(row + (tid < g.head ? tid : g.nvec * EPV + tid) * E::kSize);
+  watch.ready();
+  if (tid < nscalar) watch.one(xs, tid);
+  float m_ref = xs;
+  auto raise = [&](const u32x4& raw, uint32_t v) {
+    float x[EPV];
+    unpacked(raw, x, v);
+#pragma unroll
+    for (int j = 0; j < EPV; ++j) m_ref = fmaxf(m_ref, x[j]);
+  };
+  if (tid < rest) raise(pong[0], whole * kStep + tid);
+  if (whole > 0) raise(ping[0], tid);
+  acc.init(wave_max(m_ref), c_scaled, kLog2e);
+  if (tid < nscalar) acc.one(xs, 0);
+  if (rest > 0) {
+    float m[kStepVecs] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+    for (uint32_t u = 0; u < kStepVecs; ++u)
+      if (u * kBlock + tid < rest) take(pong[u], m[u], whole * kStep + u * kBlock + tid);
+    if constexpr (W::kMaxima) watch.note(whole, whole, rest, m);
+  }
+  if (whole == 0) return;
+  uint32_t step = 0;
+  for (; step + 2 < whole; step += 2) {
+    load(pong, step + 1);
+    consume(ping, step);
+    load(ping, step + 2);
+    consume(pong, step + 1);
+  }
+  if (step + 1 < whole) {
+    load(pong, step + 1);
+    consume(ping, step);
+    consume(pong, step + 1);
+  } else {
+    consume(ping, step);
+  }
+}
+
 // Rows whose fast sums are not usable (an element some 88 nats above the references, logits at the
 // lowest values of their type, inf, NaN) or would lose digits (references so far from 0 that the
 // roundings of x c, which grow with |x|, reach 2^-16 and the entropy's with it): the exact maximum

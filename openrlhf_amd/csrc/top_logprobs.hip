@@ -173,7 +173,7 @@ __device__ __forceinline__ void write_skipped_row(const TopArgs& a, int64_t row_
 // eighth of the row: 221 against 208 us at 4096 x 151936 bf16, k = 64.) A row that has more candidates
 // than fit (many equal logits), or a NaN, goes through collect_row instead.
 constexpr int kMaxBlocks = 32;
-constexpr uint32_t kBlockVecs = 4;  // vectors in a block, and a thread's loads per step
+constexpr uint32_t kBlockVecs = kStepVecs;  // vectors in a block: as many as a step gives each lane
 
 // Lane j of four gets the maximum over the four lanes of m[j].
 __device__ __forceinline__ float quad_maxima(const float (&m)[4]) {
@@ -189,95 +189,25 @@ __device__ __forceinline__ float quad_maxima(const float (&m)[4]) {
   return with_neighbour(high ? hi : lo, high ? lo : hi, kSwap2);
 }
 
-// The loads of the next step are in flight while one is worked on: two steps of registers, 16 KiB
-// asked for ahead by each workgroup at any time. The vectors past the last whole step come first, so
-// that the loop has no predicated step (after one the compiler waits for every load before it issues
-// the next). The wave's exponent reference is the maximum of its lanes' first vectors.
-template <int DT, int MODE>
-__device__ __forceinline__ float stream_row(const char* row, const RowGeom& g, float c_scaled, ListAcc<MODE>& acc,
-                                            float* block_max, int shift) {
-  using E = Elt<DT>;
-  constexpr int EPV = E::kPerVec;
-  constexpr uint32_t kStep = kBlockVecs * kBlock;
-  const uint32_t tid = threadIdx.x;
-  const char* body = row + g.head * E::kSize;
-  float thread_max = -INFINITY;
-  const uint32_t whole = g.nvec / kStep, rest = g.nvec - whole * kStep;
-  auto load = [&](u32x4 (&raw)[kBlockVecs], uint32_t step) {
-    const uint32_t at = step * (kStep * 16u) + tid * 16u;
-#pragma unroll
-    for (uint32_t u = 0; u < kBlockVecs; ++u) raw[u] = load_vec(body + (at + u * (kBlock * 16u)));
-    __builtin_amdgcn_sched_barrier(0);  // all of them issued before the work on the step at hand
-  };
-  auto note = [&](uint32_t step, const float (&m)[kBlockVecs]) {
+struct BlockMaxima {
+  static constexpr bool kMaxima = true;
+  float* block_max;
+  int shift;
+  float thread_max;
+  __device__ __forceinline__ void ready() const {}
+  template <int N>
+  __device__ __forceinline__ void vec(float (&)[N], uint32_t) const {}
+  __device__ __forceinline__ void one(float&, uint32_t) const {}
+  // Maxima of a step's vectors. The remainder (step == whole) is noted first: it opens its slot, the
+  // others of the slot add to it.
+  __device__ __forceinline__ void note(uint32_t step, uint32_t whole, uint32_t rest, const float (&m)[kStepVecs]) {
     const float bm = quad_maxima(m);
-    float* slot = block_max + (step >> shift) * kBlock + tid;
-    // the remainder (step == whole) is noted first: it opens its slot, the others of the slot add to it
+    float* slot = block_max + (step >> shift) * kBlock + threadIdx.x;
     const bool opens = (step & ((1u << shift) - 1u)) == 0u && (shift == 0 || rest == 0u || (step >> shift) != (whole >> shift));
     *slot = opens || step == whole ? bm : fmaxf(*slot, bm);
     thread_max = fmaxf(thread_max, bm);
-  };
-  auto take = [&](const u32x4& raw, float& m) {
-    uint32_t w0 = raw[0], w1 = raw[1], w2 = raw[2], w3 = raw[3];
-    asm volatile("" : "+v"(w0), "+v"(w1), "+v"(w2), "+v"(w3));  // unpacked here, not ahead for several vectors
-    float x[EPV];
-    E::unpack(u32x4{w0, w1, w2, w3}, x);
-#pragma unroll
-    for (int j = 0; j < EPV; ++j) m = fmaxf(m, x[j]);
-    acc.vec(x, 0);
-    acc.settle();  // one vector's values at a time: registers decide how many rows a CU holds
-  };
-  auto consume = [&](const u32x4 (&raw)[kBlockVecs], uint32_t step) {
-    float m[kBlockVecs] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-    for (uint32_t u = 0; u < kBlockVecs; ++u) take(raw[u], m[u]);
-    note(step, m);
-  };
-  auto raise = [&](const u32x4& raw, float& m) {
-    float x[EPV];
-    E::unpack(raw, x);
-#pragma unroll
-    for (int j = 0; j < EPV; ++j) m = fmaxf(m, x[j]);
-  };
-
-  u32x4 ping[kBlockVecs], pong[kBlockVecs];
-#pragma unroll
-  for (uint32_t u = 0; u < kBlockVecs; ++u)
-    if (u * kBlock + tid < rest) pong[u] = load_vec(body + (whole * kStep + u * kBlock + tid) * 16u);
-  if (whole > 0) load(ping, 0);
-  // head and tail of a row off the 16-byte grid: at most one element per thread
-  const uint32_t nscalar = g.head + g.tail;
-  float xs = -INFINITY;
-  if (tid < nscalar) xs = E::load1(row + (tid < g.head ? tid : g.nvec * EPV + tid) * E::kSize);
-  float m_ref = xs;
-  if (tid < rest) raise(pong[0], m_ref);
-  if (whole > 0) raise(ping[0], m_ref);
-  acc.init(wave_max(m_ref), c_scaled, kLog2e);
-  if (tid < nscalar) acc.one(xs, 0);
-  if (rest > 0) {
-    float m[kBlockVecs] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-    for (uint32_t u = 0; u < kBlockVecs; ++u)
-      if (u * kBlock + tid < rest) take(pong[u], m[u]);
-    note(whole, m);
   }
-  if (whole == 0) return thread_max;
-  uint32_t step = 0;
-  for (; step + 2 < whole; step += 2) {
-    load(pong, step + 1);
-    consume(ping, step);
-    load(ping, step + 2);
-    consume(pong, step + 1);
-  }
-  if (step + 1 < whole) {
-    load(pong, step + 1);
-    consume(ping, step);
-    consume(pong, step + 1);
-  } else {
-    consume(ping, step);
-  }
-  return thread_max;
-}
+};
 
 // The largest value of 16 leading bits that at least k of the 256 values reach: one wave, four values
 // per lane, one counting step per bit.
@@ -471,8 +401,9 @@ __global__ __launch_bounds__(kBlock) void top_logprobs_fwd_kernel(TopArgs a) {
     if (at >= 0 && at < seg.len) x_label = E::load1(row + at * E::kSize);
   }
   ListAcc<MODE> acc;
-  const float thread_max = stream_row<DT, MODE>(row, g, (float)(1.4426950408889634 / a.temperature), acc, block_max, a.shift);
-  sh.best[tid] = ordered_bits(thread_max);
+  BlockMaxima maxima = {block_max, a.shift, -INFINITY};
+  stream_row<DT, MODE>(row, g, (float)(1.4426950408889634 / a.temperature), acc, maxima);
+  sh.best[tid] = ordered_bits(maxima.thread_max);
   const RowSums sums = combine_fast<MODE>(acc, sh.lds);  // its barriers also publish the maxima
   RowTotals totals;
   if (fast_usable<MODE>(sums)) {
@@ -491,7 +422,7 @@ __global__ __launch_bounds__(kBlock) void top_logprobs_fwd_kernel(TopArgs a) {
   __syncthreads();
   const uint32_t bits = sh.bar_bits;
   const float bar = bits <= ordered_bits(-INFINITY) ? -INFINITY : ordered_value(bits);
-  collect_blocks<DT>(row, g, seg.first, block_max, a.shift, bar, thread_max, sh.list, cand);
+  collect_blocks<DT>(row, g, seg.first, block_max, a.shift, bar, maxima.thread_max, sh.list, cand);
   __syncthreads();
   int n = cand.count;
   if (n > kCap || sh.list.count > kListed || nan) {

@@ -11,7 +11,8 @@ plus ``logprobs_and_entropy_from_logits``, the one-pass form of what Actor.forwa
 two calls (openrlhf/models/actor.py:269-285), and ``lm_head_logprobs_and_entropy``, the same from
 the last hidden states and the lm_head weight with the logits never stored
 (openrlhf/models/actor.py:263-285). ``top_logprobs_from_logits`` adds the k most likely tokens of
-every position to the one-pass form (no reference counterpart).
+every position to the one-pass form, and ``distill_kl_from_logits`` / ``fused_distill_kl_fwd_bwd`` are
+the loss of a student on such a list of its teacher's (no reference counterpart).
 
 Every function launches hand-written HIP kernels through the C ABI; tensors must be on the GPU.
 
@@ -237,15 +238,6 @@ def _list_workspace(ws_bytes, n_rows, dev):
     return ws, None if torch.cuda.is_current_stream_capturing() else _row_tickets(dev, n_rows)
 
 
-def _f32_rows(t, shape, name):
-    """Contiguous fp32 [prod(shape)] of a per-row tensor, or None."""
-    if t is None:
-        return None
-    if t.shape != shape:
-        raise ValueError(f"{name} shape {tuple(t.shape)} != {tuple(shape)}")
-    return t.to(torch.float32).contiguous()
-
-
 class _TopLogprobs(torch.autograd.Function):
     """logits -> (log-prob of label, entropy, log-probs of the k most likely tokens, their ids)."""
 
@@ -335,6 +327,158 @@ def top_logprobs_from_logits(
     ``inplace_backward`` and ``row_mask`` as in ``logprobs_and_entropy_from_logits``; a position with
     mask 0 gets ids -1 and zeros."""
     return _TopLogprobs.apply(logits, labels, int(k), temperature, bool(return_entropy), inplace_backward, row_mask)
+
+
+# ------------------------------------------------------------------ distillation from a teacher's top tokens
+def _distill_kind(kl, tail):
+    if kl == "forward":
+        return _lib.DISTILL_FORWARD_TAIL if tail else _lib.DISTILL_FORWARD
+    if kl != "reverse":
+        raise ValueError(f"Unknown kl: {kl} (forward or reverse)")
+    if not tail:
+        raise ValueError("the reverse KL needs the teacher's tail (tail=True): without it the divergence is infinite")
+    return _lib.DISTILL_REVERSE_TAIL
+
+
+class _DistillCall:
+    """One distillation call's arguments, checked and laid out as the kernels take them."""
+
+    def __init__(self, logits, teacher_ids, teacher_log_probs, temperature, kl, tail, teacher_temperature, row_mask):
+        self.dev = require_gpu(logits, teacher_ids, teacher_log_probs, row_mask)
+        self.code = _lib.dtype_code(logits)
+        self.kind = _distill_kind(kl, tail)
+        if self.kind != _lib.DISTILL_FORWARD and teacher_temperature != 1.0:
+            raise ValueError("teacher_temperature applies to tail=False; with a tail the teacher's log-probs are taken as they are")
+        self.batch_shape = logits.shape[:-1]
+        if teacher_ids.shape != teacher_log_probs.shape or teacher_ids.shape[:-1] != self.batch_shape or teacher_ids.dim() != logits.dim():
+            raise ValueError(f"teacher_ids {tuple(teacher_ids.shape)} and teacher_log_probs {tuple(teacher_log_probs.shape)} "
+                             f"must both be {tuple(self.batch_shape)} + (k,)")
+        if teacher_ids.dtype not in (torch.int64, torch.int32):
+            raise TypeError(f"teacher_ids must be int64 or int32, got {teacher_ids.dtype}")
+        self.k = teacher_ids.shape[-1]
+        if not 1 <= self.k <= _lib.LIST_MAX:
+            raise ValueError(f"the teacher's list has {self.k} entries per position, 1..{_lib.LIST_MAX} are supported")
+        self.rows, self.row_stride, self.aliases = _as_rows(logits.detach())
+        self.n_rows, self.vocab = self.rows.shape
+        self.logits_shape = logits.shape
+        self.ids = teacher_ids.to(torch.int64).contiguous()
+        self.teacher = teacher_log_probs.detach().to(torch.float32).contiguous()
+        self.rmask = _mask_rows(row_mask, self.batch_shape)
+        self.temperature, self.teacher_temperature = float(temperature), float(teacher_temperature)
+
+    def forward(self, keep):
+        """Per-row loss and, with ``keep``, what the backward needs."""
+        opts = dict(device=self.dev, dtype=torch.float32)
+        loss = torch.empty(self.n_rows, **opts)
+        stats = torch.empty((self.n_rows, 4), **opts) if keep else None
+        list_grad = torch.empty((self.n_rows, self.k), **opts) if keep else None
+        list_at = torch.empty((self.n_rows, self.k), device=self.dev, dtype=torch.int32) if keep else None
+        with _lib.on_device(self.dev):
+            ws_bytes = _lib.load().orlhf_distill_kl_workspace_bytes(self.code, self.n_rows, self.vocab)
+            ws, tickets = _list_workspace(ws_bytes, self.n_rows, self.dev)
+            call("orlhf_distill_kl_fwd", ptr(self.rows), self.code, self.n_rows, self.vocab, self.row_stride, ptr(self.ids),
+                 ptr(self.teacher), self.k, self.temperature, self.teacher_temperature, self.kind, ptr(loss), ptr(stats),
+                 ptr(list_grad), ptr(list_at), ptr(self.rmask), ptr(ws), ws_bytes, ptr(tickets), stream_of(self.dev))
+        return loss, (stats, list_grad, list_at)
+
+
+def _distill_backward(rows, row_stride, k, temperature, g_loss, saved, rmask, inplace):
+    """d loss / d logits rows from what the forward kept; over the logits when ``inplace``."""
+    stats, list_grad, list_at = saved
+    n_rows, vocab = rows.shape
+    if inplace:
+        grad_rows, grad_stride = rows, row_stride
+    else:
+        grad_rows, grad_stride = torch.empty((n_rows, vocab), device=rows.device, dtype=rows.dtype), vocab
+    with _lib.on_device(rows.device):
+        call("orlhf_distill_kl_bwd", ptr(rows), ptr(grad_rows), _lib.dtype_code(rows), n_rows, vocab, row_stride, grad_stride,
+             k, temperature, ptr(g_loss), ptr(stats), ptr(list_grad), ptr(list_at), ptr(rmask), stream_of(rows.device))
+    if inplace:  # as in _LogprobEntropy: the logits are gone
+        torch.autograd.graph.increment_version(rows)
+    return grad_rows
+
+
+class _DistillKL(torch.autograd.Function):
+    """(logits, teacher's list) -> KL divergence per position."""
+
+    @staticmethod
+    def forward(ctx, logits, teacher_ids, teacher_log_probs, temperature, kl, tail, teacher_temperature, inplace_backward, row_mask):
+        c = _DistillCall(logits, teacher_ids, teacher_log_probs, temperature, kl, tail, teacher_temperature, row_mask)
+        needs_grad = ctx.needs_input_grad[0]
+        loss, saved = c.forward(needs_grad)
+        ctx.k, ctx.temperature, ctx.row_stride = c.k, c.temperature, c.row_stride
+        ctx.inplace = bool(inplace_backward) and c.aliases
+        ctx.logits_shape = logits.shape
+        if needs_grad:
+            ctx.save_for_backward(c.rows, c.rmask, *saved)
+        return loss.view(c.batch_shape)
+
+    @staticmethod
+    def backward(ctx, g_loss):
+        rows, rmask, *saved = ctx.saved_tensors
+        g = g_loss.to(torch.float32).contiguous()
+        grad = _distill_backward(rows, ctx.row_stride, ctx.k, ctx.temperature, g, saved, rmask, ctx.inplace)
+        return (grad if grad.shape == ctx.logits_shape else grad.view(ctx.logits_shape),) + (None,) * 8
+
+
+def distill_kl_from_logits(
+    logits: torch.Tensor,
+    teacher_ids: torch.Tensor,
+    teacher_log_probs: torch.Tensor,
+    temperature: float = 1.0,
+    kl: str = "forward",
+    tail: bool = True,
+    teacher_temperature: float = 1.0,
+    inplace_backward: bool = False,
+    row_mask: Optional[torch.Tensor] = None,
+) -> torch.Tensor:
+    """KL divergence per position between a teacher known by its most likely tokens and the student
+    ``q = softmax(logits / temperature)``; fp32, differentiable in the logits.
+
+    ``teacher_ids`` (int64 or int32) and ``teacher_log_probs``, both ``[..., k]`` with ``k <= 128``, are
+    what ``top_logprobs_from_logits(teacher_logits, None, k, temperature)`` returns. With p the teacher's
+    probabilities, t = 1 - sum p and s the student's probability of everything outside the list:
+
+      * ``kl="forward", tail=True``: ``sum p log(p / q) + t log(t / s)``, the divergence of the two
+        distributions over the listed tokens and one outcome for the rest;
+      * ``kl="forward", tail=False``: ``sum w log(w / q)`` with w the teacher renormalised over its
+        list, ``softmax(teacher_log_probs / teacher_temperature)`` (logits will do), against the
+        student's full softmax;
+      * ``kl="reverse", tail=True``: ``sum q log(q / p) + s log(s / t)`` (t at least 2^-24).
+
+    Entries with a negative id or a log-prob of -inf are absent (ragged lists); an id that comes twice
+    counts once with the sum of its probabilities; an id past the vocabulary makes the position's loss
+    NaN. Positions without an entry, or with ``row_mask`` 0, have loss 0 and no gradient.
+    ``inplace_backward=True`` writes the gradient over the logits storage, as in
+    ``logprobs_and_entropy_from_logits``."""
+    return _DistillKL.apply(logits, teacher_ids, teacher_log_probs, temperature, kl, tail, teacher_temperature,
+                            inplace_backward, row_mask)
+
+
+@torch.no_grad()
+def fused_distill_kl_fwd_bwd(
+    logits: torch.Tensor,
+    teacher_ids: torch.Tensor,
+    teacher_log_probs: torch.Tensor,
+    weights: torch.Tensor,
+    temperature: float = 1.0,
+    kl: str = "forward",
+    tail: bool = True,
+    teacher_temperature: float = 1.0,
+    inplace: bool = True,
+    row_mask: Optional[torch.Tensor] = None,
+) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Forward and backward of ``sum(weights * distill_kl_from_logits(...))`` for weights ``[...]`` known
+    up front (``mask / n_tokens``). Returns ``(loss [...], d / d logits)``; with ``inplace=True`` the
+    gradient overwrites the logits storage. Not an autograd function: the gradient is returned."""
+    require_gpu(logits, weights)
+    c = _DistillCall(logits, teacher_ids, teacher_log_probs, temperature, kl, tail, teacher_temperature, row_mask)
+    if weights.shape != c.batch_shape:
+        raise ValueError(f"weights shape {tuple(weights.shape)} != logits batch shape {tuple(c.batch_shape)}")
+    w = weights.to(torch.float32).contiguous()
+    loss, saved = c.forward(True)
+    grad = _distill_backward(c.rows, c.row_stride, c.k, c.temperature, w, saved, c.rmask, inplace and c.aliases)
+    return loss.view(c.batch_shape), grad if grad.shape == logits.shape else grad.view(logits.shape)
 
 
 # ------------------------------------------------------------------ lm-head + log-prob, logits not stored

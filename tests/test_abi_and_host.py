@@ -376,3 +376,46 @@ def test_top_logprobs_entries_refuse_bad_arguments(lib):
     assert bwd(gh=8, gs=63) == -1 and "grad_row_stride" in err()
     with pytest.raises(RuntimeError, match="GPU only"):
         top_logprobs_from_logits(torch.zeros(2, 8), None, 2)
+
+
+def test_distill_entries_refuse_bad_arguments(lib):
+    import torch
+
+    from openrlhf_amd import _lib
+    from openrlhf_amd.models.utils import _distill_kind, distill_kl_from_logits
+
+    def err():
+        return lib.orlhf_last_error().decode()
+
+    fwd = lambda x=8, dt=1, n=2, v=64, stride=64, ids=8, lp=8, k=4, t=1.0, tt=1.0, kind=0, loss=8, st=None, lg=None, at=None, ws=None, nb=0, tick=None: (  # noqa: E731
+        lib.orlhf_distill_kl_fwd(x, dt, n, v, stride, ids, lp, k, t, tt, kind, loss, st, lg, at, None, ws, nb, tick, None))
+    for k in (0, 129):
+        assert fwd(k=k) == -1 and "k=" in err()
+    assert fwd(stride=63) == -1 and "row_stride" in err()
+    assert fwd(v=520193, stride=520193) == -3 and "not implemented" in err()
+    for t in (0.0, -1.0, float("nan"), float("inf")):
+        assert fwd(t=t) == -1 and "temperature" in err()
+        assert fwd(kind=1, tt=t) == -1 and "teacher_temperature" in err()
+    assert fwd(kind=0, tt=2.0) == -1 and "tail" in err()
+    assert fwd(kind=3) == -1 and "kind" in err()
+    assert fwd(dt=4) == -1 and "dtype" in err()
+    for bad in (dict(x=None), dict(ids=None), dict(lp=None), dict(loss=None)):
+        assert fwd(**bad) == -1 and "NULL" in err()
+    assert fwd(st=8) == -1 and "go together" in err()
+    assert fwd(x=9) == -1 and "aligned" in err()
+    assert fwd(tick=2) == -1 and "tickets" in err()
+    need = lib.orlhf_distill_kl_workspace_bytes(1, 2, 151936)
+    assert need > 0 and lib.orlhf_distill_kl_workspace_bytes(1, 4096, 151936) == 0
+    assert fwd(v=151936, stride=151936, ws=8, nb=need - 1) == -1 and "workspace" in err()
+    assert fwd(n=0, x=None) == 0
+    bwd = lambda gs=64, g=8, at=8: lib.orlhf_distill_kl_bwd(8, 8, 1, 2, 64, 64, gs, 4, 1.0, g, 8, 8, at, None, None)  # noqa: E731
+    assert bwd(gs=63) == -1 and "grad_row_stride" in err()
+    assert bwd(g=None) == -1 and "NULL" in err()
+    assert bwd(at=None) == -1 and "NULL" in err()
+    assert _distill_kind("forward", False) == _lib.DISTILL_FORWARD
+    with pytest.raises(ValueError, match="Unknown kl"):
+        _distill_kind("js", True)
+    with pytest.raises(ValueError, match="infinite"):
+        _distill_kind("reverse", False)
+    with pytest.raises(RuntimeError, match="GPU only"):
+        distill_kl_from_logits(torch.zeros(2, 8), torch.zeros(2, 1, dtype=torch.long), torch.zeros(2, 1))

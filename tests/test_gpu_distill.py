@@ -1,0 +1,287 @@
+"""distill_kl_from_logits and fused_distill_kl_fwd_bwd against the definition in float64 (a Python sum
+over outcomes per row, differentiated by autograd), and the pair of operators as they are used.
+
+Bounds, u = 2^-24. The student's sum outside the list is relatively within rel = (V / 1024 + 3 X c + 24) u
+of the exact one (its terms carry the rounding of their exponents, of which X = max |x| and
+c = log2(e) / T set the size, and its accumulators one rounding per term); everything after it runs in
+fp64. The loss depends on it through log s and the log-sum-exp, with derivatives of at most 2 (forward)
+or 2 + |log-ratios| (reverse), and is rounded once."""
+import math
+
+import pytest
+import torch
+
+from oracle import vocab_lists as ov
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+TYPES = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
+FLOOR = {torch.bfloat16: 1e-37, torch.float16: 2.0 ** -25, torch.float32: 1e-37}
+FORMS = [("forward", True), ("forward", False), ("reverse", True)]
+
+
+def _case(rows, vocab, k, dtype, seed, pad=0, offset=0, sharp=14.0, ragged=False):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(rows, vocab, generator=g) * 2
+    x[torch.arange(rows), torch.randint(0, vocab, (rows,), generator=g)] += sharp * torch.rand(rows, generator=g)
+    store = torch.empty(rows * (vocab + pad) + offset, dtype=TYPES[dtype], device="cuda")
+    view = store[offset:].view(rows, vocab + pad)[:, :vocab]
+    view.copy_(x.to(TYPES[dtype]))
+    teacher = x * 0.8 + torch.randn(rows, vocab, generator=g)
+    top = torch.topk(torch.log_softmax(teacher.double(), -1), k, dim=1)
+    ids, lps = top.indices, top.values.float()
+    if ragged:
+        gone = torch.arange(k)[None] >= torch.randint(0, k + 1, (rows, 1), generator=g)
+        ids[gone] = -1
+        lps[gone & (torch.rand(rows, k, generator=g) < 0.5)] = -math.inf
+    return view, ids, lps, g
+
+
+def _reference(view, ids, lps, temperature, form, rows, teacher_temperature=1.0):
+    out = []
+    for r in rows:
+        x = view[r].detach().double().cpu().requires_grad_(True)
+        loss = ov.distill_kl_row(x, ids[r], lps[r].double(), temperature, teacher_temperature, *form)
+        (grad,) = torch.autograd.grad(loss, [x])
+        out.append((loss.item(), grad, x.detach()))
+    return out
+
+
+def _check(view, ids, lps, temperature, form, loss, grad=None, weight=None, rows=None, teacher_temperature=1.0):
+    rows = range(view.shape[0]) if rows is None else rows
+    c = math.log2(math.e) / temperature
+    for r, (want, d, x) in zip(rows, _reference(view, ids, lps, temperature, form, rows, teacher_temperature)):
+        fin = x[x.abs() < 1e30]
+        big = fin.abs().max().item()
+        rel = (x.numel() / 1024 + 3 * big * c + 24) * U
+        lt = lps[r][(ids[r] >= 0) & (lps[r] > -math.inf)].double().abs()
+        ratios = 2 + (lt.max().item() if lt.numel() else 0.0) + 2 * big / temperature if form[0] == "reverse" else 2.0
+        got = loss[r].item()
+        assert abs(got - want) <= ratios * rel + 2 * U * abs(want), (r, got, want)
+        if grad is not None:
+            w = weight[r].item()
+            lq = torch.log_softmax(x / temperature, -1)
+            q = lq.exp()
+            # d / d(log s), d / d(lse) of the coefficient of q: |d| itself, and t / s in the forward form with
+            # the tail; a listed entry is a difference of terms up to q and p, rounded in fp32
+            slack = 2 * rel + 4 * U * (lq.abs().clamp(max=100) + 4)
+            listed = torch.zeros_like(q)
+            on = (ids[r] >= 0) & (lps[r] > -math.inf)
+            listed[ids[r][on]] = lps[r][on].double().exp()
+            bound = (d.abs() * temperature + q * ratios) * slack / temperature + 4 * U * listed / temperature
+            if form == ("forward", True) and on.any():
+                outside = (listed == 0)
+                s = q[outside].sum().clamp(min=2.0 ** -126)
+                t = max(0.0, 1.0 - listed.sum().item())
+                bound = bound + (t / s) * q * outside * 4 * rel / temperature
+            bound = bound * abs(w)
+            half = torch.finfo(grad.dtype).eps / 2
+            err = (grad[r].double().cpu() - w * d).abs()
+            assert (err <= half * (abs(w) * d.abs() + bound) + bound + FLOOR[grad.dtype]).all(), (r, (err - bound).max())
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("rows,vocab,k,dtype,temperature,pad,offset,ragged", [
+    (1, 1, 1, "fp32", 1.0, 0, 0, False),
+    (3, 2, 1, "bf16", 0.5, 0, 1, False),
+    (4, 9, 9, "fp32", 1.0, 0, 0, False),
+    (5, 131, 128, "fp16", 1.0, 1, 3, True),
+    (8, 1000, 20, "bf16", 0.7, 0, 0, True),
+    (6, 5003, 65, "fp32", 2.0, 5, 3, True),
+    (3, 32000, 1, "fp16", 1.0, 0, 0, False),
+    (3, 50257, 128, "bf16", 1.5, 6, 1, True),
+    (2, 151936, 64, "bf16", 1.0, 0, 0, False),
+    (1, 262144, 50, "fp32", 1.0, 0, 0, True),
+    (1, 520192, 20, "fp16", 0.8, 0, 0, False),
+    (514, 4099, 7, "bf16", 1.0, 0, 0, True),
+])
+def test_loss_and_gradients(cuda, form, rows, vocab, k, dtype, temperature, pad, offset, ragged):
+    from openrlhf_amd.models.utils import distill_kl_from_logits, fused_distill_kl_fwd_bwd
+
+    view, ids, lps, g = _case(rows, vocab, k, dtype, 7 * rows + vocab + k, pad, offset, ragged=ragged)
+    scale = 64.0 if dtype == "fp16" else 1.0  # fp16 gradients of a wide row need a scaled loss
+    weight = (0.2 + torch.rand(rows, generator=g)) * scale
+    few = range(rows) if rows < 20 else [0, 1, rows - 1]
+    leaf = view.detach().requires_grad_(True)
+    loss = distill_kl_from_logits(leaf, ids.cuda(), lps.cuda(), temperature, *form)
+    (grad,) = torch.autograd.grad([loss], [leaf], [weight.cuda()])
+    _check(view, ids, lps, temperature, form, loss.detach().cpu(), grad, weight, few)
+    for inplace in (False, True):
+        x = view.clone() if not inplace else view
+        before = view.clone()
+        loss2, grad2 = fused_distill_kl_fwd_bwd(x, ids.cuda(), lps.cuda(), weight.cuda(), temperature, *form, inplace=inplace)
+        assert (grad2.data_ptr() == x.data_ptr()) == inplace
+        _check(before, ids, lps, temperature, form, loss2.cpu(), grad2, weight, few)
+        if not inplace:
+            assert torch.equal(x, before)
+
+
+@pytest.mark.parametrize("form", FORMS)
+def test_gradient_against_differences(cuda, form):
+    from openrlhf_amd.models.utils import distill_kl_from_logits
+
+    view, ids, lps, _ = _case(3, 30, 5, "fp32", 4, sharp=2.0)
+    leaf = view.detach().requires_grad_(True)
+    loss = distill_kl_from_logits(leaf, ids.cuda(), lps.cuda(), 1.3, *form)
+    (grad,) = torch.autograd.grad(loss.sum(), [leaf])
+    h = 1e-5
+    for r, j in [(0, int(ids[0, 0])), (0, 7), (1, int(ids[1, 4])), (2, 29)]:
+        x = view[r].double().cpu()
+        d = torch.zeros_like(x)
+        d[j] = h
+        f = lambda y: ov.distill_kl_row(y, ids[r], lps[r].double(), 1.3, 1.0, *form).item()  # noqa: E731
+        # truncation h^2, rounding 1e-14 / h, the kernel's fp32
+        assert abs((f(x + d) - f(x - d)) / (2 * h) - grad[r, j].item()) <= 1e-8 + 1e-5 * (1 + abs(grad[r, j].item()))
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("vocab", [400, 40011])
+def test_lists_with_absent_repeated_and_foreign_ids(cuda, form, vocab):
+    from openrlhf_amd.models.utils import distill_kl_from_logits
+
+    view, ids, lps, _ = _case(7, vocab, 6, "fp32", 13)
+    lps = lps - 1.0           # leaves mass for the tail
+    ids[1] = -1               # nothing listed
+    lps[2] = -math.inf        # nothing listed either
+    ids[3, 4] = ids[3, 1]     # one id twice
+    ids[4, :] = ids[4, 0]     # one id six times
+    lps[4] = torch.tensor([-3.0, -2.5, -4.0, -3.0, -6.0, -2.7])
+    ids[5, 2] = vocab         # past the vocabulary
+    ids[6, 3], lps[6, 5] = -7, -math.inf
+    leaf = view.detach().requires_grad_(True)
+    loss = distill_kl_from_logits(leaf, ids.cuda().int(), lps.cuda(), 1.0, *form)
+    weight = torch.ones(7)
+    (grad,) = torch.autograd.grad(loss.sum(), [leaf])
+    _check(view, ids, lps, 1.0, form, loss.detach().cpu(), grad, weight, [0, 1, 2, 3, 4, 6])
+    assert loss[1].item() == 0 and loss[2].item() == 0 and (grad[1:3] == 0).all()
+    assert math.isnan(loss[5].item()) and grad[5].isfinite().all()  # the foreign id has no gradient, the others do
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("vocab", [600, 33000])
+def test_sure_students_and_masked_vocabularies(cuda, form, dtype, vocab):
+    """Rows where 1 - sum q would be rounding noise, and rows whose other logits are masked."""
+    from openrlhf_amd.models.utils import distill_kl_from_logits
+
+    g = torch.Generator().manual_seed(1)
+    x = torch.randn(6, vocab, generator=g)
+    ids = torch.stack([torch.randperm(vocab, generator=g)[:4] for _ in range(6)])
+    lps = torch.log(torch.tensor([[0.6, 0.25, 0.1, 0.04]])).repeat(6, 1)
+    at = torch.arange(6)
+    x[at, ids[:, 0]] += torch.tensor([5.0, 25.0, 40.0, 70.0, 0.0, 120.0])  # student's mass elsewhere: 1e-2 ... 1e-49
+    keep = torch.zeros(vocab, dtype=torch.bool)
+    keep[ids[4]] = True
+    x[4, ~keep] = torch.finfo(TYPES[dtype]).min  # everything outside the list is masked
+    x = x.to(TYPES[dtype])
+    leaf = x.cuda().requires_grad_(True)
+    loss = distill_kl_from_logits(leaf, ids.cuda(), lps.cuda(), 1.0, *form)
+    (grad,) = torch.autograd.grad(loss.sum(), [leaf])
+    assert loss.isfinite().all() and grad.isfinite().all()
+    _check(x.cuda(), ids, lps, 1.0, form, loss.detach().cpu(), grad, torch.ones(6), [0, 1, 2, 3])
+    _check(x.cuda(), ids, lps, 1.0, form, loss.detach().cpu(), None, None, [4, 5])
+    low = x.clone()
+    low[0, keep.logical_not()] = -math.inf
+    low[0, ids[0]] = x[0, ids[0]]
+    out = distill_kl_from_logits(low[:1].cuda(), ids[:1].cuda(), lps[:1].cuda(), 1.0, *form)
+    assert out.isfinite().all()
+
+
+def test_masked_rows_weights_of_zero_and_teacher_temperature(cuda):
+    from openrlhf_amd.models.utils import distill_kl_from_logits, fused_distill_kl_fwd_bwd
+
+    view, ids, lps, g = _case(30, 6001, 9, "bf16", 3)
+    mask = torch.rand(30, generator=g) < 0.5
+    mask[0], mask[1] = True, False
+    poison = view.clone()
+    poison[~mask.cuda()] = math.nan  # masked rows are not read
+    leaf = poison.requires_grad_(True)
+    loss = distill_kl_from_logits(leaf, ids.cuda(), lps.cuda(), row_mask=mask.cuda())
+    weight = torch.rand(30, generator=g)
+    weight[0] = 0.0
+    (grad,) = torch.autograd.grad([loss], [leaf], [weight.cuda()])
+    assert (loss[~mask.cuda()] == 0).all() and (grad[~mask.cuda()] == 0).all() and (grad[0] == 0).all()
+    rows = mask.nonzero()[:, 0].tolist()
+    _check(view, ids, lps, 1.0, ("forward", True), loss.detach().cpu(), grad, weight, rows)
+    loss2, grad2 = fused_distill_kl_fwd_bwd(poison.detach().clone(), ids.cuda(), lps.cuda(), weight.cuda(), row_mask=mask.cuda().float())
+    assert (loss2[~mask.cuda()] == 0).all() and (grad2[~mask.cuda()] == 0).all() and (grad2[0] == 0).all()
+    _check(view, ids, lps, 1.0, ("forward", True), loss2.cpu(), grad2, weight, rows)
+    raw = lps * 3 + 5  # logits of the teacher, at a temperature
+    loss3 = distill_kl_from_logits(view, ids.cuda(), raw.cuda(), 1.4, tail=False, teacher_temperature=2.5)
+    _check(view, ids, raw, 1.4, ("forward", False), loss3.cpu(), rows=range(5), teacher_temperature=2.5)
+
+
+def test_shapes_dtypes_and_empty_batches(cuda):
+    from openrlhf_amd.models.utils import distill_kl_from_logits
+
+    view, ids, lps, _ = _case(6, 515, 5, "bf16", 2)
+    want = distill_kl_from_logits(view, ids.cuda(), lps.cuda())
+    x = view.reshape(2, 3, 515)
+    got = distill_kl_from_logits(x, ids.view(2, 3, 5).cuda().int(), lps.view(2, 3, 5).cuda().double())
+    assert got.shape == (2, 3) and torch.equal(got.view(-1), want)
+    turned = x.permute(0, 2, 1).contiguous().permute(0, 2, 1)
+    assert torch.equal(distill_kl_from_logits(turned, ids.view(2, 3, 5).cuda(), lps.view(2, 3, 5).cuda()).view(-1), want)
+    assert distill_kl_from_logits(view[:0], ids[:0].cuda(), lps[:0].cuda()).shape == (0,)
+
+
+@pytest.mark.parametrize("rows,vocab,dtype", [(1, 151936, "bf16"), (9, 50257, "fp16"), (300, 70001, "bf16")])
+def test_cut_rows_merged_in_one_launch_or_two_give_the_same_bits(cuda, rows, vocab, dtype):
+    from openrlhf_amd import _lib
+
+    view, ids, lps, _ = _case(rows, vocab, 33, dtype, rows, ragged=True)
+    if rows > 3:
+        view[0, 5] = math.nan
+        view[1] = -math.inf
+        view[2] = torch.finfo(TYPES[dtype]).min
+    code = _lib.dtype_code(view)
+    mask = torch.ones(rows, dtype=torch.uint8, device="cuda")
+    mask[rows // 2 : rows // 2 + rows // 5] = 0
+    nbytes = _lib.load().orlhf_distill_kl_workspace_bytes(code, rows, vocab)
+    assert nbytes > 0
+    tickets = torch.zeros(rows, dtype=torch.int32, device="cuda")
+    idc, lpc = ids.cuda(), lps.cuda()
+
+    def once(tick, kind):
+        ws = torch.randint(0, 255, (nbytes,), dtype=torch.uint8, device="cuda")
+        loss, stats = torch.full((rows,), 7.0, device="cuda"), torch.full((rows, 4), 7.0, device="cuda")
+        lg, at = torch.full((rows, 33), 7.0, device="cuda"), torch.full((rows, 33), 7, device="cuda", dtype=torch.int32)
+        _lib.call("orlhf_distill_kl_fwd", view.data_ptr(), code, rows, vocab, vocab, idc.data_ptr(), lpc.data_ptr(), 33, 0.9, 1.0,
+                  kind, loss.data_ptr(), stats.data_ptr(), lg.data_ptr(), at.data_ptr(), mask.data_ptr(), ws.data_ptr(), nbytes,
+                  None if tick is None else tick.data_ptr(), _lib.stream_of(view.device))
+        return [t.view(torch.int32) for t in (loss, stats, lg, at)]
+
+    for kind in (_lib.DISTILL_FORWARD_TAIL, _lib.DISTILL_FORWARD, _lib.DISTILL_REVERSE_TAIL):
+        want = once(None, kind)
+        for _ in range(8):
+            got = once(tickets, kind)
+            assert int(tickets.abs().sum()) == 0
+            for a, b in zip(got, want):
+                assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("rows", [3, 600])
+def test_other_stream_and_replayed_graph_give_the_same_bits(cuda, rows):
+    from openrlhf_amd.models.utils import distill_kl_from_logits, fused_distill_kl_fwd_bwd
+
+    view, ids, lps, g = _case(rows, 30011, 12, "bf16", 9)
+    other, ids2, lps2, _ = _case(rows, 30011, 12, "bf16", 10)
+    w = torch.rand(rows, generator=g).cuda()
+    args = lambda i, p: (i.cuda(), p.cuda(), w)  # noqa: E731
+    want = fused_distill_kl_fwd_bwd(view, *args(ids, lps), inplace=False)
+    want2 = fused_distill_kl_fwd_bwd(other, *args(ids2, lps2), inplace=False)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        again = fused_distill_kl_fwd_bwd(view, *args(ids, lps), inplace=False)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(again[0], want[0]) and torch.equal(again[1], want[1])
+    sx, si, sl = view.clone(), ids.cuda(), lps.cuda()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = fused_distill_kl_fwd_bwd(sx, si, sl, w, inplace=False)
+    for x, i, p, expect in ((other, ids2, lps2, want2), (view, ids, lps, want), (other, ids2, lps2, want2)):
+        sx.copy_(x), si.copy_(i), sl.copy_(p)
+        graph.replay()
+        distill_kl_from_logits(view, ids.cuda(), lps.cuda(), 0.5)  # eager work between the replays
+        torch.cuda.synchronize()
+        assert torch.equal(out[0], expect[0]) and torch.equal(out[1], expect[1])
