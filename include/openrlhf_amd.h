@@ -237,6 +237,22 @@ int orlhf_distill_kl_bwd(const void* logits, void* grad_logits, int dtype, int64
                          orlhf_stream_t stream);
 
 /*
+ * Both in one pass for callers that know the upstream weights when the forward runs (loss = sum_i
+ * weight[i] * loss[i]): computes loss as orlhf_distill_kl_fwd and writes d / d logits as
+ * orlhf_distill_kl_bwd with g_loss = weight (a row of weight 0 is read, for its loss, and its gradient is
+ * 0). Every row is read once and written once. `grad_logits` may alias `logits` (same row stride); rows
+ * of both have to sit on the same 16-byte phase and vocab may be at most
+ * orlhf_distill_kl_fwd_bwd_max_vocab(dtype) (ORLHF_ERR_UNSUPPORTED otherwise: use the two entries).
+ */
+int64_t orlhf_distill_kl_fwd_bwd_max_vocab(int dtype);
+int orlhf_distill_kl_fwd_bwd(const void* logits, void* grad_logits, int dtype, int64_t n_rows,
+                             int64_t vocab, int64_t row_stride, int64_t grad_row_stride,
+                             const int64_t* teacher_ids, const float* teacher_logprob, int64_t k,
+                             double temperature, double teacher_temperature, int kind,
+                             const float* weight, float* loss, const uint8_t* row_mask,
+                             orlhf_stream_t stream);
+
+/*
  * Forward and backward in ONE pass for callers that know the upstream weights when the forward
  * runs, i.e. whose loss is sum_i w_logprob[i]*logprob[i] + w_entropy[i]*entropy[i] (SFT:
  * w_logprob = -mask/N, openrlhf/models/loss.py:104): computes logprob / entropy exactly as

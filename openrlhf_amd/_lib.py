@@ -91,6 +91,8 @@ SIGNATURES = {
     "orlhf_distill_kl_fwd": (c_int, [P, c_int, I64, I64, I64, P, P, I64, c_double, c_double, c_int, P, P, P, P, P, P, I64, P,
                                      P]),
     "orlhf_distill_kl_bwd": (c_int, [P, P, c_int, I64, I64, I64, I64, I64, c_double, P, P, P, P, P, P]),
+    "orlhf_distill_kl_fwd_bwd_max_vocab": (I64, [c_int]),
+    "orlhf_distill_kl_fwd_bwd": (c_int, [P, P, c_int, I64, I64, I64, I64, P, P, I64, c_double, c_double, c_int, P, P, P, P]),
     "orlhf_lmhead_workspace_bytes": (I64, [I64, I64, I64, I64, c_int]),
     "orlhf_lmhead_logprob_entropy_fwd": (c_int, [P, P, c_int, I64, I64, I64, I64, I64, P, c_double, P, P, P, P, I64, I64,
                                                  P, I64, P]),

@@ -200,28 +200,6 @@ static int launch_distill_bwd(const DistillBwdArgs& a, hipStream_t stream) {
   return ORLHF_OK;
 }
 
-static int check_distill(const char* what, int dtype, int64_t n_rows, int64_t vocab, int64_t row_stride, int64_t k,
-                         double temperature) {
-  ORLHF_CHECK_ARG(n_rows >= 0 && vocab > 0, "%s: n_rows=%lld vocab=%lld", what, (long long)n_rows, (long long)vocab);
-  ORLHF_CHECK_ARG(row_stride >= vocab, "%s: row_stride %lld < vocab %lld", what, (long long)row_stride, (long long)vocab);
-  if (vocab > kMaxDistillVocab)
-    return fail(ORLHF_ERR_UNSUPPORTED, "%s: vocab %lld, rows beyond %lld elements are not implemented", what,
-                (long long)vocab, (long long)kMaxDistillVocab);
-  ORLHF_CHECK_ARG(temperature > 0.0 && temperature < INFINITY, "%s: temperature must be > 0 and finite", what);
-  ORLHF_CHECK_ARG(dtype == ORLHF_F32 || dtype == ORLHF_BF16 || dtype == ORLHF_F16, "%s: unknown dtype %d", what, dtype);
-  ORLHF_CHECK_ARG(k >= 1 && k <= kMaxList, "%s: k=%lld must lie in 1..%d", what, (long long)k, kMaxList);
-  return ORLHF_OK;
-}
-
-static int check_kind(const char* what, int kind, double teacher_temperature) {
-  ORLHF_CHECK_ARG(kind >= ORLHF_DISTILL_FORWARD_TAIL && kind <= ORLHF_DISTILL_REVERSE_TAIL, "%s: unknown kind %d", what, kind);
-  ORLHF_CHECK_ARG(teacher_temperature > 0.0 && teacher_temperature < INFINITY,
-                  "%s: teacher_temperature must be > 0 and finite", what);
-  ORLHF_CHECK_ARG(kind == ORLHF_DISTILL_FORWARD || teacher_temperature == 1.0,
-                  "%s: a kind with a tail takes log-probs as they are (teacher_temperature 1)", what);
-  return ORLHF_OK;
-}
-
 }  // namespace orlhf
 
 using namespace orlhf;

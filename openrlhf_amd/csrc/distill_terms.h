@@ -38,21 +38,34 @@ struct ListSource {
   double inv_teacher_t;
 };
 
+// The row's list as it stands in memory.
+struct RawList {
+  int64_t id[2];
+  float value[2];
+};
+__device__ __forceinline__ RawList fetch_list(const ListSource& src, int64_t row_i) {
+  RawList raw;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int at = (int)(threadIdx.x & (kWave - 1)) + i * kWave;
+    raw.id[i] = at < src.k ? src.ids[row_i * src.k + at] : -1;
+    raw.value[i] = at < src.k ? src.teacher[row_i * src.k + at] : -INFINITY;
+  }
+  return raw;
+}
+
 template <int DT>
-__device__ __forceinline__ ListEntries load_list(const ListSource& src, int64_t row_i, const char* row, int64_t vocab) {
+__device__ __forceinline__ ListEntries settle_list(const RawList& raw, const ListSource& src, const char* row, int64_t vocab) {
   using E = Elt<DT>;
   const int lane = threadIdx.x & (kWave - 1);
   ListEntries e;
   e.bad = false;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    const int at = lane + i * kWave;
-    const int64_t id = at < src.k ? src.ids[row_i * src.k + at] : -1;
-    const float v = at < src.k ? src.teacher[row_i * src.k + at] : -INFINITY;
-    const bool given = id >= 0 && v != -INFINITY;
-    e.bad = e.bad || (given && id >= vocab);
-    e.id[i] = given && id < vocab ? (int)id : -1;
-    e.lp[i] = (double)v * src.inv_teacher_t;
+    const bool given = raw.id[i] >= 0 && raw.value[i] != -INFINITY;
+    e.bad = e.bad || (given && raw.id[i] >= vocab);
+    e.id[i] = given && raw.id[i] < vocab ? (int)raw.id[i] : -1;
+    e.lp[i] = (double)raw.value[i] * src.inv_teacher_t;
     e.x[i] = e.id[i] >= 0 ? E::load1(row + (int64_t)e.id[i] * E::kSize) : 0.0f;
   }
   e.bad = __ballot(e.bad) != 0ull;
@@ -86,6 +99,11 @@ __device__ __forceinline__ ListEntries load_list(const ListSource& src, int64_t 
   return e;
 }
 
+template <int DT>
+__device__ __forceinline__ ListEntries load_list(const ListSource& src, int64_t row_i, const char* row, int64_t vocab) {
+  return settle_list<DT>(fetch_list(src, row_i), src, row, vocab);
+}
+
 // One bit per element of a row (or segment), set for the listed ones, in the order of the body's
 // elements: a vector of 8 elements is a byte, one of 4 half a byte. The scalars at the row's ends have
 // bits of their own behind it.
@@ -111,6 +129,10 @@ struct ListMap {
       atomicOr(words + (i - g.head) / 32u, 1u << ((i - g.head) % 32u));
     }
   }
+  // Takes an element's bit, and those around it, out again (all bits set are taken out this way).
+  __device__ __forceinline__ void drop(const RowGeom& g, uint32_t i) const {
+    if (i >= g.head && i - g.head < g.nvec * EPV) words[(i - g.head) / 32u] = 0u;
+  }
   __device__ __forceinline__ uint32_t vec(uint32_t v) const {
     const uint8_t* b = (const uint8_t*)words;
     return EPV == 8 ? b[v] : (uint32_t)(b[v >> 1] >> ((v & 1u) * 4u)) & 0xfu;
@@ -125,7 +147,7 @@ struct WithoutListed {
   template <int N>
   __device__ __forceinline__ void vec(float (&x)[N], uint32_t v) const {
     const uint32_t bits = map.vec(v);
-    if (bits != 0u) {
+    if (__ballot(bits != 0u) != 0ull) {  // a branch of the wave, hardly ever taken
 #pragma unroll
       for (int j = 0; j < N; ++j) x[j] = (bits >> j & 1u) != 0u ? -INFINITY : x[j];
     }
@@ -213,7 +235,8 @@ __device__ __forceinline__ ListTerms list_terms(const ListEntries& e, const RowT
   r.l2 = (float)((log_total + (at - (double)r.centre) / temperature) * 1.4426950408889634);
   if (n_on == 0) {  // nothing to learn from: no loss, no gradient
     r.loss = r.other = 0.0;
-    r.centre = r.l2 = 0.0f;
+    r.centre = INFINITY;  // every weight of the backward 0
+    r.l2 = 0.0f;
   }
   if (e.bad) r.loss = NAN;
   return r;
@@ -223,6 +246,29 @@ __device__ __forceinline__ ListTerms list_terms(const ListEntries& e, const RowT
 __device__ __forceinline__ float grad_coef(double upstream, double other, double temperature) {
   const double a = upstream * other / temperature;
   return (float)(a > 3.0e38 ? 3.0e38 : (a < -3.0e38 ? -3.0e38 : a));
+}
+
+// ---------------------------------------------------------------- host side
+inline int check_distill(const char* what, int dtype, int64_t n_rows, int64_t vocab, int64_t row_stride, int64_t k,
+                         double temperature) {
+  ORLHF_CHECK_ARG(n_rows >= 0 && vocab > 0, "%s: n_rows=%lld vocab=%lld", what, (long long)n_rows, (long long)vocab);
+  ORLHF_CHECK_ARG(row_stride >= vocab, "%s: row_stride %lld < vocab %lld", what, (long long)row_stride, (long long)vocab);
+  if (vocab > kMaxDistillVocab)
+    return fail(ORLHF_ERR_UNSUPPORTED, "%s: vocab %lld, rows beyond %lld elements are not implemented", what,
+                (long long)vocab, (long long)kMaxDistillVocab);
+  ORLHF_CHECK_ARG(temperature > 0.0 && temperature < INFINITY, "%s: temperature must be > 0 and finite", what);
+  ORLHF_CHECK_ARG(dtype == ORLHF_F32 || dtype == ORLHF_BF16 || dtype == ORLHF_F16, "%s: unknown dtype %d", what, dtype);
+  ORLHF_CHECK_ARG(k >= 1 && k <= kMaxList, "%s: k=%lld must lie in 1..%d", what, (long long)k, kMaxList);
+  return ORLHF_OK;
+}
+
+inline int check_kind(const char* what, int kind, double teacher_temperature) {
+  ORLHF_CHECK_ARG(kind >= ORLHF_DISTILL_FORWARD_TAIL && kind <= ORLHF_DISTILL_REVERSE_TAIL, "%s: unknown kind %d", what, kind);
+  ORLHF_CHECK_ARG(teacher_temperature > 0.0 && teacher_temperature < INFINITY,
+                  "%s: teacher_temperature must be > 0 and finite", what);
+  ORLHF_CHECK_ARG(kind == ORLHF_DISTILL_FORWARD || teacher_temperature == 1.0,
+                  "%s: a kind with a tail takes log-probs as they are (teacher_temperature 1)", what);
+  return ORLHF_OK;
 }
 
 }  // namespace orlhf

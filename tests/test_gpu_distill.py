@@ -94,6 +94,12 @@ def _check(view, ids, lps, temperature, form, loss, grad=None, weight=None, rows
     (1, 262144, 50, "fp32", 1.0, 0, 0, True),
     (1, 520192, 20, "fp16", 0.8, 0, 0, False),
     (514, 4099, 7, "bf16", 1.0, 0, 0, True),
+    (700, 151936, 64, "bf16", 1.0, 0, 0, False),
+    (300, 262144, 100, "fp16", 0.7, 0, 0, True),
+    (530, 50257, 128, "fp32", 1.0, 6, 3, True),
+    (1031, 33, 33, "fp32", 1.3, 3, 1, True),
+    (260, 80001, 11, "fp32", 2.0, 0, 0, False),
+    (257, 520192, 20, "bf16", 1.0, 0, 0, True),
 ])
 def test_loss_and_gradients(cuda, form, rows, vocab, k, dtype, temperature, pad, offset, ragged):
     from openrlhf_amd.models.utils import distill_kl_from_logits, fused_distill_kl_fwd_bwd
@@ -101,7 +107,7 @@ def test_loss_and_gradients(cuda, form, rows, vocab, k, dtype, temperature, pad,
     view, ids, lps, g = _case(rows, vocab, k, dtype, 7 * rows + vocab + k, pad, offset, ragged=ragged)
     scale = 64.0 if dtype == "fp16" else 1.0  # fp16 gradients of a wide row need a scaled loss
     weight = (0.2 + torch.rand(rows, generator=g)) * scale
-    few = range(rows) if rows < 20 else [0, 1, rows - 1]
+    few = range(rows) if rows < 20 else [0, 1, rows // 2, rows - 2, rows - 1]
     leaf = view.detach().requires_grad_(True)
     loss = distill_kl_from_logits(leaf, ids.cuda(), lps.cuda(), temperature, *form)
     (grad,) = torch.autograd.grad([loss], [leaf], [weight.cuda()])
@@ -187,21 +193,23 @@ def test_sure_students_and_masked_vocabularies(cuda, form, dtype, vocab):
     assert out.isfinite().all()
 
 
-def test_masked_rows_weights_of_zero_and_teacher_temperature(cuda):
+@pytest.mark.parametrize("n", [30, 1200])
+def test_masked_rows_weights_of_zero_and_teacher_temperature(cuda, n):
     from openrlhf_amd.models.utils import distill_kl_from_logits, fused_distill_kl_fwd_bwd
 
-    view, ids, lps, g = _case(30, 6001, 9, "bf16", 3)
-    mask = torch.rand(30, generator=g) < 0.5
+    view, ids, lps, g = _case(n, 6001, 9, "bf16", 3)
+    mask = torch.rand(n, generator=g) < 0.5
     mask[0], mask[1] = True, False
     poison = view.clone()
     poison[~mask.cuda()] = math.nan  # masked rows are not read
     leaf = poison.requires_grad_(True)
     loss = distill_kl_from_logits(leaf, ids.cuda(), lps.cuda(), row_mask=mask.cuda())
-    weight = torch.rand(30, generator=g)
+    weight = torch.rand(n, generator=g)
     weight[0] = 0.0
     (grad,) = torch.autograd.grad([loss], [leaf], [weight.cuda()])
     assert (loss[~mask.cuda()] == 0).all() and (grad[~mask.cuda()] == 0).all() and (grad[0] == 0).all()
     rows = mask.nonzero()[:, 0].tolist()
+    rows = rows[:12] + rows[-12:]
     _check(view, ids, lps, 1.0, ("forward", True), loss.detach().cpu(), grad, weight, rows)
     loss2, grad2 = fused_distill_kl_fwd_bwd(poison.detach().clone(), ids.cuda(), lps.cuda(), weight.cuda(), row_mask=mask.cuda().float())
     assert (loss2[~mask.cuda()] == 0).all() and (grad2[~mask.cuda()] == 0).all() and (grad2[0] == 0).all()
@@ -209,6 +217,59 @@ def test_masked_rows_weights_of_zero_and_teacher_temperature(cuda):
     raw = lps * 3 + 5  # logits of the teacher, at a temperature
     loss3 = distill_kl_from_logits(view, ids.cuda(), raw.cuda(), 1.4, tail=False, teacher_temperature=2.5)
     _check(view, ids, raw, 1.4, ("forward", False), loss3.cpu(), rows=range(5), teacher_temperature=2.5)
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("vocab,dtype", [(900, "fp32"), (151937, "bf16"), (200003, "fp16")])
+def test_one_pass_on_rows_that_go_wrong(cuda, form, vocab, dtype):
+    """The one-pass kernel against the two kernels on a batch that mixes ordinary rows with sure students,
+    masked vocabularies, lists that are empty, repeated or out of range, -inf, NaN and far-off logits, so
+    that a row's state must not leak into the rows its workgroup takes next."""
+    from openrlhf_amd.models.utils import _DistillCall, _distill_backward, fused_distill_kl_fwd_bwd
+
+    rows = 1100
+    view, ids, lps, g = _case(rows, vocab, 10, dtype, 77, pad=8 - vocab % 8 if vocab % 8 else 0, ragged=True)
+    kind = torch.arange(rows) % 11
+    low = torch.finfo(TYPES[dtype]).min
+    lps = lps - 0.5
+    dev = lambda m: m.cuda()  # noqa: E731
+    view[dev(kind == 1)] += 300.0 if dtype != "fp16" else 200.0
+    spot = ids[:, 0].clamp(min=0).cuda()
+    view[dev(kind == 2), spot[dev(kind == 2)]] = 90.0
+    ids[kind == 3] = -1
+    ids[kind == 4, 3] = ids[kind == 4, 0]
+    ids[kind == 5, 2] = vocab + 5
+    view[dev(kind == 6), : vocab - 3] = low
+    view[dev(kind == 7)] = -math.inf
+    view[dev(kind == 8), 11] = math.nan
+    view[dev(kind == 9), 7 : vocab // 2] = -math.inf
+    mask = (torch.rand(rows, generator=g) < 0.8).cuda()
+    weight = torch.rand(rows, generator=g).cuda()
+    weight[::13] = 0.0
+    idc, lpc = ids.cuda(), lps.cuda()
+    c = _DistillCall(view, idc, lpc, 0.9, *form, 1.0, mask)
+    want, saved = c.forward(True)
+    want_grad = _distill_backward(c.rows, c.row_stride, c.k, c.temperature, weight, saved, c.rmask, False)
+    got, grad = fused_distill_kl_fwd_bwd(view.clone(memory_format=torch.preserve_format) if vocab % 8 == 0 else view, idc, lpc,
+                                         weight, 0.9, *form, inplace=True, row_mask=mask)
+    finite = want.isfinite()
+    assert torch.equal(got.isfinite(), finite) and torch.equal(got.isnan(), want.isnan())
+    live = ((kind != 7) & (kind != 8)).cuda() & mask  # rows without a softmax: NaN in both
+    # sums of the same terms in another order: twice the bound of each; far-off logits take the exact path
+    rel = 4 * (vocab / 1024 + 3 * 64 * 2 + 24) * U
+    close = (got - want).abs() <= 4 * rel * (1 + want.abs())
+    assert close[finite].all(), (kind.cuda()[finite & ~close], (got - want)[finite & ~close])
+    a, b = grad[live].float(), want_grad[live].float()
+    half = torch.finfo(TYPES[dtype]).eps / 2
+    assert a.isfinite().all() and b.isfinite().all()
+    # an element that is not listed: a product, each factor within 4 rel. A listed one is a difference of
+    # terms up to w / T, of which the student's, q, moves by q times the change of the log-sum-exp (rel)
+    # (reverse: times the log-ratio, up to 2 X / T, as well)
+    listed = torch.zeros_like(b, dtype=torch.bool).scatter_(1, idc[live].clamp(0, vocab - 1), True)
+    size = 1.0 if form[0] == "forward" else 1.0 + 2 * 100 / 0.9
+    tol = (2 * half + 8 * rel) * b.abs() + listed * (rel * size * weight[live][:, None] / 0.9) + 2 * FLOOR[TYPES[dtype]]
+    assert ((a - b).abs() <= tol).all(), (((a - b).abs() - tol).max(), kind[live.cpu()][((a - b).abs() > tol).any(1).cpu()])
+    assert (grad[~mask] == 0).all() and (grad[::13][live[::13]] == 0).all()
 
 
 def test_shapes_dtypes_and_empty_batches(cuda):
