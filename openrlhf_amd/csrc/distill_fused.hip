@@ -48,9 +48,15 @@ struct ListTable {
   int* key;  // [kSlots], -1: free
   float* value;
   static __device__ __forceinline__ uint32_t slot_of(int id) { return ((uint32_t)id * 2654435761u) >> 24; }
-  __device__ __forceinline__ int insert(int id) const {
+  // The slot of an id: its own, where another lane has put the same id already (`repeated`).
+  __device__ __forceinline__ int insert(int id, bool& repeated) const {
     uint32_t s = slot_of(id);
-    for (int n = 0; n < kSlots && atomicCAS(key + s, -1, id) != -1; ++n) s = (s + 1u) % kSlots;  // 128 of 256 taken at most
+    for (int n = 0; n < kSlots; ++n) {  // 128 of 256 taken at most
+      const int was = atomicCAS(key + s, -1, id);
+      repeated = was == id;
+      if (was == -1 || repeated) break;
+      s = (s + 1u) % kSlots;
+    }
     return (int)s;
   }
   __device__ __forceinline__ float find(int id) const {
@@ -62,12 +68,13 @@ struct ListTable {
 
 // A row's list while the row is on chip: one wave's, kept in LDS because the row has the registers.
 struct ListState {
-  double lp[kMaxList];
+  double lp[kMaxList], p[kMaxList];
   float x[kMaxList];
   int id[kMaxList], slot[kMaxList];
-  uint32_t head, nvec;  // of the row
+  double mass, t, log_t, log_mass, top, sum;  // TeacherTerms, StudentTerms
+  uint32_t head, nvec;                        // of the row
   float weight;
-  int bad;
+  int n_on, bad;
 };
 
 // Workgroup barrier for what passes through LDS: loads and stores of device memory stay in flight.
@@ -99,7 +106,8 @@ __global__ __launch_bounds__(kOneBlock) void distill_one_pass_kernel(OneArgs a) 
   extern __shared__ u32x4 maps[];  // two maps, then the parked chunks
   u32x4(*const park)[kOneBlock] = (u32x4(*)[kOneBlock])(maps + a.map_words / 2);
   const uint32_t tid = threadIdx.x, tid16 = tid * 16u, lane = tid % kWave, wave = tid / kWave;
-  const float cT = (float)(1.4426950408889634 / a.temperature);
+  const double inv_t = 1.0 / a.temperature;
+  const float cT = (float)(1.4426950408889634 * inv_t);
 
   // next row of this workgroup that is wanted; `write`: unwanted rows on the way get their zeros
   auto next_active = [&](int64_t r, bool write) -> int64_t {
@@ -139,10 +147,12 @@ __global__ __launch_bounds__(kOneBlock) void distill_one_pass_kernel(OneArgs a) 
   };
 
   // Wave 0: a row's list into the map, table and state of side `to`, which the list of two rows ago leaves.
-  auto mark = [&](int64_t row, const RowGeom& gn, int to) {
+  auto mark = [&](const RawList& raw, int64_t row, const RowGeom& gn, int to) {
     const ListMap<DT> map = {(uint32_t*)maps + to * a.map_words, ends + to};
     const ListTable table = {keys[to], values[to]};
     ListState& st = state[to];
+    ListEntries e = settle_list<DT>(raw, a.list, a.logits + row * a.row_stride_bytes, a.vocab);
+    const float weight = a.weight[row];
     const RowGeom old = {st.head, st.nvec, 0u};
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -155,27 +165,49 @@ __global__ __launch_bounds__(kOneBlock) void distill_one_pass_kernel(OneArgs a) 
       }
     }
     if (lane == 0) *map.ends = 0u;
-    const ListEntries e = load_list<DT>(a.list, row, a.logits + row * a.row_stride_bytes, a.vocab);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the old entries are out before the new ones go in
+    bool repeated = false;
+    int slot[2] = {0, 0};
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int id = e.id[i], at = (int)lane + i * kWave;
-      st.id[at] = id;
-      st.x[at] = e.x[i];
-      st.lp[at] = e.lp[i];
+      const int id = e.id[i];
       if (id >= 0) {
+        bool again;
+        slot[i] = table.insert(id, again);
+        repeated = repeated || again;
         map.set(gn, id, a.vocab);
-        st.slot[at] = table.insert(id);
         uint32_t* d = dirty_of(to, gn, (uint32_t)id);
         if (d != nullptr) atomicOr(d, 1u << (chunk_of(gn, (uint32_t)id) % 32u));
       }
     }
+    if (__ballot(repeated) != 0ull) join_repeats(e, a.list.k);
+    const TeacherTerms t = teacher_terms(e, a.kind, a.vocab);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int at = (int)lane + i * kWave;
+      st.id[at] = e.id[i];
+      st.slot[at] = slot[i];
+      st.x[at] = e.x[i];
+      st.lp[at] = e.lp[i];
+      st.p[at] = t.p[i];
+    }
     if (lane == 0) {
-      st.head = gn.head;
-      st.nvec = gn.nvec;
-      st.weight = a.weight[row];
+      st.mass = t.mass, st.t = t.t, st.log_t = t.log_t, st.log_mass = t.log_mass, st.n_on = t.n_on;
+      st.head = gn.head, st.nvec = gn.nvec;
+      st.weight = weight;
       st.bad = e.bad ? 1 : 0;
     }
+  };
+  auto listed = [&](int at) {  // of one wave
+    ListEntries e;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      e.id[i] = state[at].id[lane + i * kWave];
+      e.x[i] = state[at].x[lane + i * kWave];
+      e.lp[i] = state[at].lp[lane + i * kWave];
+    }
+    e.bad = state[at].bad != 0;
+    return e;
   };
 
   if (row_i < a.n_rows) {  // prologue: the first row's loads, then its list
@@ -188,7 +220,7 @@ __global__ __launch_bounds__(kOneBlock) void distill_one_pass_kernel(OneArgs a) 
     if (tid < g.head + g.tail) xs = E::load1(row + (tid < g.head ? tid : g.nvec * EPV + tid) * E::kSize);
   }
   __syncthreads();  // the empty maps and tables
-  if (row_i < a.n_rows && wave == 0) mark(row_i, g, 0);
+  if (row_i < a.n_rows && wave == 0) mark(fetch_list(a.list, row_i), row_i, g, 0);
   lds_barrier();
 
   while (row_i < a.n_rows) {
@@ -232,6 +264,11 @@ __global__ __launch_bounds__(kOneBlock) void distill_one_pass_kernel(OneArgs a) 
         }
       }
     };
+
+    if (TAIL && wave == 1) {  // the listed logits' own sum, while the row's loads land
+      const StudentTerms t = student_terms(listed(side), inv_t);
+      if (lane == 0) state[side].top = t.top, state[side].sum = t.sum;
+    }
 
     // ---- sum against the wave maximum of each lane's first chunk (it lands first)
     float ref;
@@ -300,16 +337,11 @@ __global__ __launch_bounds__(kOneBlock) void distill_one_pass_kernel(OneArgs a) 
     // ---- the row's loss and gradient coefficients (one wave, fp64)
     const int64_t next_i = next_active(row_i + gridDim.x, false);
     if (wave == 0) {
-      const float w = state[side].weight;
-      ListEntries list;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        list.id[i] = state[side].id[lane + i * kWave];
-        list.x[i] = state[side].x[lane + i * kWave];
-        list.lp[i] = state[side].lp[lane + i * kWave];
-      }
-      list.bad = state[side].bad != 0;
-      const ListTerms t = list_terms(list, totals, a.kind, a.temperature, a.vocab);
+      const ListState& st = state[side];
+      const float w = st.weight;
+      const ListEntries list = listed(side);
+      const TeacherTerms teacher = {{st.p[lane], st.p[lane + kWave]}, st.mass, st.t, st.log_t, st.log_mass, st.n_on};
+      const ListTerms t = list_terms(list, teacher, StudentTerms{st.top, st.sum}, totals, a.kind, a.temperature, a.vocab);
       if (lane == 0) {
         a.loss[row_i] = (float)t.loss;
         bcast[0] = w == 0.0f ? INFINITY : t.centre;  // weight 0: every exponent -inf, every gradient 0
@@ -335,6 +367,8 @@ __global__ __launch_bounds__(kOneBlock) void distill_one_pass_kernel(OneArgs a) 
     };
 
     // ---- gradient of this row out, next row in, chunk by chunk through the same registers
+    RawList raw;
+    if (next_i < a.n_rows && wave == 0) raw = fetch_list(a.list, next_i);
     if (a.row_mask != nullptr) next_active(row_i + gridDim.x, true);
     const bool has_next = next_i < a.n_rows;
     const char* nrow = a.logits + (has_next ? next_i : row_i) * a.row_stride_bytes;
@@ -367,7 +401,7 @@ __global__ __launch_bounds__(kOneBlock) void distill_one_pass_kernel(OneArgs a) 
     }
     xs = -INFINITY;
     if (tid < gn.head + gn.tail) xs = E::load1(nrow + (tid < gn.head ? tid : gn.nvec * EPV + tid) * E::kSize);
-    if (has_next && wave == 0) mark(next_i, gn, side ^ 1);
+    if (has_next && wave == 0) mark(raw, next_i, gn, side ^ 1);
     lds_barrier();
     row_i = next_i;
     g = gn;

@@ -69,39 +69,53 @@ __device__ __forceinline__ ListEntries settle_list(const RawList& raw, const Lis
     e.x[i] = e.id[i] >= 0 ? E::load1(row + (int64_t)e.id[i] * E::kSize) : 0.0f;
   }
   e.bad = __ballot(e.bad) != 0ull;
-  bool again[2] = {false, false};  // the id stands earlier in the list
+  return e;
+}
+
+// Whether an id stands in the list more than once.
+__device__ __forceinline__ bool list_repeats(const ListEntries& e, int k) {
+  const int lane = threadIdx.x & (kWave - 1);
+  bool again = false;
 #pragma unroll 1
-  for (int j = 0; j < src.k - 1; ++j) {
+  for (int j = 0; j < k - 1; ++j) {
     const int other = j < kWave ? __builtin_amdgcn_readlane(e.id[0], j) : __builtin_amdgcn_readlane(e.id[1], j - kWave);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) again[i] = again[i] || (e.id[i] == other && other >= 0 && lane + i * kWave > j);
+    for (int i = 0; i < 2; ++i) again = again || (e.id[i] == other && other >= 0 && lane + i * kWave > j);
   }
-  if (__ballot(again[0] || again[1]) != 0ull) {  // rare: add the later ones to the first
-    double sum[2] = {exp(e.lp[0]), exp(e.lp[1])};
+  return __ballot(again) != 0ull;
+}
+
+// Adds the probabilities of an id's later entries to its first, in their order, and drops them.
+__device__ __forceinline__ void join_repeats(ListEntries& e, int k) {
+  const int lane = threadIdx.x & (kWave - 1);
+  double sum[2] = {exp(e.lp[0]), exp(e.lp[1])};
+  bool more[2] = {false, false}, again[2] = {false, false};
 #pragma unroll 1
-    for (int j = 1; j < src.k; ++j) {
-      const bool second = j >= kWave;
-      const int other = __shfl(second ? e.id[1] : e.id[0], j & (kWave - 1), kWave);
-      const double lp = __shfl(second ? e.lp[1] : e.lp[0], j & (kWave - 1), kWave);
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-        if (other >= 0 && e.id[i] == other && lane + i * kWave < j) sum[i] += exp(lp);
-    }
+  for (int j = 0; j < k; ++j) {
+    const bool second = j >= kWave;
+    const int other = __shfl(second ? e.id[1] : e.id[0], j & (kWave - 1), kWave);
+    const double lp = __shfl(second ? e.lp[1] : e.lp[0], j & (kWave - 1), kWave);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const double joint = log(sum[i]);
-      if (e.id[i] >= 0 && joint > e.lp[i]) e.lp[i] = joint;
+      const int at = lane + i * kWave;
+      if (other >= 0 && e.id[i] == other && at != j) {
+        if (at < j) sum[i] += exp(lp), more[i] = true;
+        if (at > j) again[i] = true;
+      }
     }
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-      if (again[i]) e.id[i] = -1;
   }
-  return e;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    if (more[i]) e.lp[i] = log(sum[i]);
+    if (again[i]) e.id[i] = -1;
+  }
 }
 
 template <int DT>
 __device__ __forceinline__ ListEntries load_list(const ListSource& src, int64_t row_i, const char* row, int64_t vocab) {
-  return settle_list<DT>(fetch_list(src, row_i), src, row, vocab);
+  ListEntries e = settle_list<DT>(fetch_list(src, row_i), src, row, vocab);
+  if (list_repeats(e, src.k)) join_repeats(e, src.k);
+  return e;
 }
 
 // One bit per element of a row (or segment), set for the listed ones, in the order of the body's
@@ -166,6 +180,45 @@ __device__ __forceinline__ double wave_max(double v) {
   return v;
 }
 
+// What the loss takes from the teacher alone and from the student's listed logits alone: each one wave's
+// work that does not wait for the row.
+struct TeacherTerms {
+  double p[2];  // of this lane's entries, 0 where absent
+  double mass, t, log_t, log_mass;
+  int n_on;
+};
+__device__ __forceinline__ TeacherTerms teacher_terms(const ListEntries& e, int kind, int64_t vocab) {
+  TeacherTerms r;
+  r.n_on = 0;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    r.n_on += __popcll(__ballot(e.id[i] >= 0));
+    r.p[i] = e.id[i] >= 0 ? exp(e.lp[i]) : 0.0;
+  }
+  r.mass = wave_sum(r.p[0] + r.p[1]);
+  const bool tail = kind != ORLHF_DISTILL_FORWARD && r.n_on < vocab;
+  r.t = tail ? fmax(1.0 - r.mass, kind == ORLHF_DISTILL_REVERSE_TAIL ? kTinyTail : 0.0) : 0.0;
+  r.log_t = log(r.t);  // used where t > 0
+  r.log_mass = kind == ORLHF_DISTILL_FORWARD ? log(r.mass) : 0.0;
+  return r;
+}
+
+struct StudentTerms {
+  double top, sum;  // sum exp(x / T - top) over the list
+};
+__device__ __forceinline__ StudentTerms student_terms(const ListEntries& e, double inv_t) {
+  double z[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) z[i] = e.id[i] >= 0 ? (double)e.x[i] * inv_t : -INFINITY;
+  StudentTerms r;
+  r.top = wave_max(z[0] > z[1] ? z[0] : z[1]);
+  double own = 0.0;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) own += e.id[i] >= 0 ? (z[i] == r.top ? 1.0 : exp(z[i] - r.top)) : 0.0;
+  r.sum = wave_sum(own);
+  return r;
+}
+
 struct ListTerms {
   double loss, other;  // the loss and dL/dz / q of an element that is not listed
   double grad[2];      // dL/dz of this lane's entries (0 where absent)
@@ -173,73 +226,64 @@ struct ListTerms {
 };
 
 // One wave. `sum`: the student's softmax sum, without the listed elements for the kinds with a tail, of
-// the whole row for the other. All of it in fp64: a few hundred operations of one wave per row.
-__device__ __forceinline__ ListTerms list_terms(const ListEntries& e, const RowTotals& sum, int kind, double temperature,
-                                                int64_t vocab) {
-  const bool tail = kind != ORLHF_DISTILL_FORWARD;
+// the whole row for the other. fp64: a few hundred operations of one wave per row.
+__device__ __forceinline__ ListTerms list_terms(const ListEntries& e, const TeacherTerms& teacher, const StudentTerms& student,
+                                                const RowTotals& sum, int kind, double temperature, int64_t vocab) {
   ListTerms r;
-  double z[2], p[2], lq[2], q[2];
-  int n_on = 0;
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const bool on = e.id[i] >= 0;
-    n_on += __popcll(__ballot(on));
-    z[i] = on ? (double)e.x[i] / temperature : -INFINITY;
-    p[i] = on ? exp(e.lp[i]) : 0.0;
-  }
-  const double mass = wave_sum(p[0] + p[1]);
+  const double inv_t = 1.0 / temperature;
+  const bool tail = kind != ORLHF_DISTILL_FORWARD;
   const bool some = sum.sT > 0.0 || sum.sT != sum.sT;  // anything of weight outside the list
   double base = some ? sum.base_t : -INFINITY, total = sum.sT;
   if (tail) {
-    const double top = wave_max(z[0] > z[1] ? z[0] : z[1]);
-    if (top > base) base = top;
-    double e01 = 0.0;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) e01 += e.id[i] >= 0 ? exp(z[i] - base) : 0.0;
-    total = (some ? sum.sT * exp(sum.base_t - base) : 0.0) + wave_sum(e01);
+    const double rest_base = base;
+    if (student.top > base) base = student.top;
+    const double listed = student.sum * (student.top == base ? 1.0 : exp(student.top - base));
+    total = (some ? sum.sT * (rest_base == base ? 1.0 : exp(rest_base - base)) : 0.0) + (teacher.n_on > 0 ? listed : 0.0);
   }
   const double log_total = sum.nan ? (double)NAN : log(total);
+  double lq[2], q[2], part[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    lq[i] = (z[i] - base) - log_total;
+    lq[i] = ((double)e.x[i] * inv_t - base) - log_total;
     q[i] = e.id[i] >= 0 ? exp(lq[i]) : 0.0;
   }
   double log_s = some ? (sum.base_t - base) + log(sum.sT) - log_total : -INFINITY;
   if (log_s < kLogTinyRest) log_s = kLogTinyRest;
-  const bool has_rest = n_on < vocab;
-  double part[2] = {0.0, 0.0};
+  const double s = exp(log_s), t = teacher.t;
   if (kind == ORLHF_DISTILL_REVERSE_TAIL) {
-    const double t = fmax(1.0 - mass, kTinyTail), log_t = log(t), s = exp(log_s);
 #pragma unroll
     for (int i = 0; i < 2; ++i) part[i] = e.id[i] >= 0 && q[i] != 0.0 ? q[i] * (lq[i] - e.lp[i]) : 0.0;
-    r.loss = wave_sum(part[0] + part[1]) + (has_rest ? s * (log_s - log_t) : 0.0);
-    r.other = (log_s - log_t) - r.loss;
+    r.loss = wave_sum(part[0] + part[1]) + (t > 0.0 ? s * (log_s - teacher.log_t) : 0.0);
+    r.other = (log_s - teacher.log_t) - r.loss;
 #pragma unroll
     for (int i = 0; i < 2; ++i) r.grad[i] = part[i] - q[i] * r.loss;
   } else {
-    const double log_mass = tail ? 0.0 : log(mass), scale = tail ? 1.0 : 1.0 / mass;
-    const double t = tail && has_rest ? fmax(1.0 - mass, 0.0) : 0.0;
+    const double scale = tail ? 1.0 : 1.0 / teacher.mass, all = tail ? teacher.mass + t : 1.0;
+    r.other = all - (t > 0.0 ? t / s : 0.0);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      p[i] *= scale;
-      part[i] = p[i] != 0.0 ? p[i] * (e.lp[i] - log_mass - lq[i]) : 0.0;
+      const double p = teacher.p[i] * scale;
+      part[i] = p != 0.0 ? p * (e.lp[i] - teacher.log_mass - lq[i]) : 0.0;
+      r.grad[i] = e.id[i] >= 0 ? all * q[i] - p : 0.0;
     }
-    r.loss = wave_sum(part[0] + part[1]) + (t > 0.0 ? t * (log(t) - log_s) : 0.0);
-    const double all = tail ? mass + t : 1.0;
-    r.other = all - (t > 0.0 ? t * exp(-log_s) : 0.0);
-#pragma unroll
-    for (int i = 0; i < 2; ++i) r.grad[i] = e.id[i] >= 0 ? all * q[i] - p[i] : 0.0;
+    r.loss = wave_sum(part[0] + part[1]) + (t > 0.0 ? t * (teacher.log_t - log_s) : 0.0);
   }
   const double at = base * temperature;
   r.centre = (float)at;
-  r.l2 = (float)((log_total + (at - (double)r.centre) / temperature) * 1.4426950408889634);
-  if (n_on == 0) {  // nothing to learn from: no loss, no gradient
+  r.l2 = (float)((log_total + (at - (double)r.centre) * inv_t) * 1.4426950408889634);
+  if (teacher.n_on == 0) {  // nothing to learn from: no loss, no gradient
     r.loss = r.other = 0.0;
     r.centre = INFINITY;  // every weight of the backward 0
     r.l2 = 0.0f;
   }
   if (e.bad) r.loss = NAN;
   return r;
+}
+
+// All of it at once.
+__device__ __forceinline__ ListTerms list_terms(const ListEntries& e, const RowTotals& sum, int kind, double temperature,
+                                                int64_t vocab) {
+  return list_terms(e, teacher_terms(e, kind, vocab), student_terms(e, 1.0 / temperature), sum, kind, temperature, vocab);
 }
 
 // Coefficient of the softmax weight in an element's gradient. A weight that is 0 has to stay 0.
