@@ -346,3 +346,26 @@ def test_other_stream_and_replayed_graph_give_the_same_bits(cuda, rows):
         distill_kl_from_logits(view, ids.cuda(), lps.cuda(), 0.5)  # eager work between the replays
         torch.cuda.synchronize()
         assert torch.equal(out[0], expect[0]) and torch.equal(out[1], expect[1])
+
+
+def test_teacher_targets_to_aggregated_student_loss(cuda):
+    """The operators as they are used: a teacher's alternatives, the student's KL on them aggregated over a
+    loss mask, and the same gradient from the one-pass form with the weights known up front."""
+    from openrlhf_amd.models.loss import aggregate_loss
+    from openrlhf_amd.models.utils import distill_kl_from_logits, fused_distill_kl_fwd_bwd, top_logprobs_from_logits
+
+    g = torch.Generator().manual_seed(12)
+    teacher = (torch.randn(4, 80, 3001, generator=g) * 2).cuda()
+    student = (teacher + torch.randn(4, 80, 3001, generator=g).cuda()).requires_grad_(True)
+    mask = (torch.rand(4, 80, generator=g) < 0.7).cuda()
+    _, _, top, ids = top_logprobs_from_logits(teacher, None, 24, return_entropy=False, row_mask=mask)
+    kl = distill_kl_from_logits(student, ids, top, row_mask=mask)
+    loss = aggregate_loss(kl, mask.float())
+    (grad,) = torch.autograd.grad(loss, [student])
+    weights = mask.float() / mask.sum()
+    kl2, grad2 = fused_distill_kl_fwd_bwd(student.detach(), ids, top, weights, inplace=False, row_mask=mask)
+    assert (kl > -1e-6).all() and (kl[~mask] == 0).all() and (ids[~mask] == -1).all()
+    # sums of the same 3001 terms in another order, logits up to 12: 2 (3 + 3 x 12 x 1.45 + 24) u, as above
+    rel = 2 * (3 + 3 * 12 * 1.45 + 24) * U
+    assert ((kl - kl2).abs() <= 4 * rel * (1 + kl.abs())).all()
+    assert ((grad - grad2).abs() <= 8 * rel * grad.abs() + 4 * rel * weights.unsqueeze(-1)).all()
