@@ -51,6 +51,7 @@ struct ListTable {
   // The slot of an id: its own, where another lane has put the same id already (`repeated`).
   __device__ __forceinline__ int insert(int id, bool& repeated) const {
     uint32_t s = slot_of(id);
+#pragma unroll 1
     for (int n = 0; n < kSlots; ++n) {  // 128 of 256 taken at most
       const int was = atomicCAS(key + s, -1, id);
       repeated = was == id;
@@ -61,6 +62,7 @@ struct ListTable {
   }
   __device__ __forceinline__ float find(int id) const {
     uint32_t s = slot_of(id);
+#pragma unroll 1
     for (int n = 0; n < kSlots && key[s] != id; ++n) s = (s + 1u) % kSlots;  // only marked ids are looked up: it is there
     return value[s];
   }
@@ -359,10 +361,16 @@ __global__ __launch_bounds__(kOneBlock) void distill_one_pass_kernel(OneArgs a) 
 #pragma unroll
       for (int j = 0; j < EPV; ++j) x[j] = grad_of(x[j]);
       if (touched(c)) {
-        const uint32_t bits = map.vec(v);
+        // one loop over the set bits: unrolled per element the look-ups made half a megabyte of code
+        uint32_t bits = map.vec(v);
+#pragma unroll 1
+        while (bits != 0u) {
+          const int at = __builtin_ctz(bits);
+          bits &= bits - 1u;
+          const float value = table.find((int)(g.head + v * EPV + at));
 #pragma unroll
-        for (int j = 0; j < EPV; ++j)
-          if ((bits >> j & 1u) != 0u) x[j] = table.find((int)(g.head + v * EPV + j));
+          for (int j = 0; j < EPV; ++j) x[j] = j == at ? value : x[j];
+        }
       }
     };
 
