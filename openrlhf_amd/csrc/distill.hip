@@ -49,8 +49,8 @@ __device__ __forceinline__ void write_skipped_list_row(const DistillArgs& a, int
   }
 }
 
-// The list is fetched, and for the kinds with a tail marked, while the row's first loads are on their way.
-template <int DT, bool TAIL>
+// The list is fetched and marked while the row's first loads are on their way.
+template <int DT>
 struct ListWatch : WithoutListed<DT> {
   static constexpr bool kMaxima = false;
   const DistillArgs* a;
@@ -59,30 +59,19 @@ struct ListWatch : WithoutListed<DT> {
   const char* row0;  // the whole row
   ListEntries* entries;  // of wave 0
   __device__ __forceinline__ void ready() const {
-    if (TAIL) {
-      this->map.clear(g, kBlock);
-      __syncthreads();
-    }
+    this->map.clear(g, kBlock);
+    __syncthreads();
     if (threadIdx.x < kWave) {
       *entries = load_list<DT>(a->list, seg.row, row0, a->vocab);
-      if (TAIL) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-          if (entries->id[i] >= 0) this->map.set(g, entries->id[i] - (int64_t)seg.first, seg.len);
-      }
+      for (int i = 0; i < 2; ++i)
+        if (entries->id[i] >= 0) this->map.set(g, entries->id[i] - (int64_t)seg.first, seg.len);
     }
-    if (TAIL) __syncthreads();
-  }
-  template <int N>
-  __device__ __forceinline__ void vec(float (&x)[N], uint32_t v) const {
-    if (TAIL) WithoutListed<DT>::vec(x, v);
-  }
-  __device__ __forceinline__ void one(float& x, uint32_t s) const {
-    if (TAIL) WithoutListed<DT>::one(x, s);
+    __syncthreads();
   }
 };
 
-template <int DT, bool TAIL>
+template <int DT>
 __global__ __launch_bounds__(kBlock) void distill_fwd_kernel(DistillArgs a) {
   using E = Elt<DT>;
   __shared__ float lds[kWavesPerBlock][8];
@@ -99,7 +88,7 @@ __global__ __launch_bounds__(kBlock) void distill_fwd_kernel(DistillArgs a) {
   const char* row = row0 + (int64_t)seg.first * E::kSize;
   const RowGeom g = row_geom<DT>(row, seg.len, false);
   ListEntries entries;
-  ListWatch<DT, TAIL> watch;
+  ListWatch<DT> watch;
   watch.map = {(uint32_t*)map_words, &ends};
   watch.a = &a, watch.g = g, watch.seg = seg, watch.row0 = row0, watch.entries = &entries;
   ListAcc<kLpOnly> acc;
@@ -180,11 +169,7 @@ template <int DT>
 static int launch_distill_fwd(const DistillArgs& a, hipStream_t stream) {
   const dim3 grid = row_grid(a.n_rows * a.split.n), block(kBlock);
   const int64_t len = a.split.n == 1 ? a.vocab : (int64_t)a.split.seg_elems;
-  if (a.kind == ORLHF_DISTILL_FORWARD) {
-    hipLaunchKernelGGL((distill_fwd_kernel<DT, false>), grid, block, 0, stream, a);
-  } else {
-    hipLaunchKernelGGL((distill_fwd_kernel<DT, true>), grid, block, (size_t)ListMap<DT>::bytes(len), stream, a);
-  }
+  hipLaunchKernelGGL((distill_fwd_kernel<DT>), grid, block, (size_t)ListMap<DT>::bytes(len), stream, a);
   ORLHF_CHECK_LAUNCH("orlhf_distill_kl_fwd");
   if (a.split.n > 1 && a.tickets == nullptr) {
     hipLaunchKernelGGL((distill_merge_kernel<DT>), row_grid(a.n_rows), dim3(kWave), 0, stream, a);

@@ -94,7 +94,7 @@ __device__ __forceinline__ u32x4 minus_inf_vec() {
   return u32x4{w, w, w, w};
 }
 
-template <int DT, int CHUNKS, bool LONG, bool TAIL>
+template <int DT, int CHUNKS, bool LONG>
 __global__ __launch_bounds__(kOneBlock) void distill_one_pass_kernel(OneArgs a) {
   using E = Elt<DT>;
   constexpr int EPV = E::kPerVec;
@@ -238,19 +238,19 @@ __global__ __launch_bounds__(kOneBlock) void distill_one_pass_kernel(OneArgs a) 
     // chunks of this lane with a listed element (the last bit: any of the streamed ones)
     const uint32_t dirty_lo = dirty[side][tid][0], dirty_hi = dirty[side][tid][1];
     auto touched = [&](int c) { return __ballot(((c < 32 ? dirty_lo : dirty_hi) >> (c % 32) & 1u) != 0u) != 0ull; };
-    // what of the row the sum sees (the kind without a tail sees all of it)
+    // what of the row the sum sees: all but the listed elements
     auto each = [&](auto&& f, auto&& settle, auto parked) {
       constexpr bool kFromLds = decltype(parked)::value;
       if (tid < nscalar) {
         float x = xs;
-        if (TAIL) without.one(x, tid);
+        without.one(x, tid);
         f(x, 0);
       }
 #pragma unroll
       for (int c = 0; c < CHUNKS; ++c) {
         float x[EPV];
         E::unpack(pinned(kFromLds && c >= CHUNKS - kParked ? park[c - (CHUNKS - kParked)][tid] : buf[c]), x);
-        if (TAIL && touched(c)) without.vec(x, (uint32_t)c * kOneBlock + tid);
+        if (touched(c)) without.vec(x, (uint32_t)c * kOneBlock + tid);
 #pragma unroll
         for (int j = 0; j < EPV; ++j) f(x[j], j & 1);
         settle();
@@ -260,14 +260,14 @@ __global__ __launch_bounds__(kOneBlock) void distill_one_pass_kernel(OneArgs a) 
         for (uint32_t v = kResident + tid; v < g.nvec; v += kOneBlock) {
           float x[EPV];
           E::unpack(*(const u32x4*)(tail_body + v * 16u), x);
-          if (TAIL) without.vec(x, v);
+          without.vec(x, v);
 #pragma unroll
           for (int j = 0; j < EPV; ++j) f(x[j], j & 1);
         }
       }
     };
 
-    if (TAIL && wave == 1) {  // the listed logits' own sum, while the row's loads land
+    if (wave == 1) {  // the listed logits' own sum, while the row's loads land
       const StudentTerms t = student_terms(listed(side), inv_t);
       if (lane == 0) state[side].top = t.top, state[side].sum = t.sum;
     }
@@ -277,7 +277,7 @@ __global__ __launch_bounds__(kOneBlock) void distill_one_pass_kernel(OneArgs a) 
     {
       float x[EPV];
       E::unpack(pinned(buf[0]), x);
-      if (TAIL && touched(0)) without.vec(x, tid);
+      if (touched(0)) without.vec(x, tid);
       ref = x[0];
 #pragma unroll
       for (int j = 1; j < EPV; ++j) ref = fmaxf(ref, x[j]);
@@ -428,14 +428,9 @@ static int launch_one_pass(const OneArgs& a, unsigned blocks, hipStream_t stream
   static_assert(2 * (kMaxMapped / 8 + 16) + kParked * kOneBlock * 16 + 18432 <= 163840, "LDS of a CU");
   const size_t lds = (size_t)a.map_words * 4 * 2 + (size_t)kParked * kOneBlock * 16;
   // more than the 64 KiB that a launch may ask for by itself
-  const void* fn = a.kind == ORLHF_DISTILL_FORWARD ? (const void*)distill_one_pass_kernel<DT, CHUNKS, LONG, false>
-                                                   : (const void*)distill_one_pass_kernel<DT, CHUNKS, LONG, true>;
-  const hipError_t e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+  const hipError_t e = hipFuncSetAttribute((const void*)distill_one_pass_kernel<DT, CHUNKS, LONG>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
   if (e != hipSuccess) return fail(ORLHF_ERR_LAUNCH, "distill_kl_fwd_bwd: %zu bytes of LDS: %s", lds, hipGetErrorString(e));
-  if (a.kind == ORLHF_DISTILL_FORWARD)
-    hipLaunchKernelGGL((distill_one_pass_kernel<DT, CHUNKS, LONG, false>), dim3(blocks), dim3(kOneBlock), lds, stream, a);
-  else
-    hipLaunchKernelGGL((distill_one_pass_kernel<DT, CHUNKS, LONG, true>), dim3(blocks), dim3(kOneBlock), lds, stream, a);
+  hipLaunchKernelGGL((distill_one_pass_kernel<DT, CHUNKS, LONG>), dim3(blocks), dim3(kOneBlock), lds, stream, a);
   ORLHF_CHECK_LAUNCH("orlhf_distill_kl_fwd_bwd");
   return ORLHF_OK;
 }

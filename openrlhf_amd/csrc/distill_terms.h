@@ -9,8 +9,9 @@
 // with P = sum p, t = 1 - P (at least 0; in the reverse form at least 2^-24, what a sum of fp32
 // probabilities resolves), s the student's mass outside the list, r = log q - log p, z = x / T. The
 // gradient of every other element is one number times q: the backward is a softmax pass and a patch of
-// the listed elements. s is summed by itself, never as 1 - sum q: for a student that is sure of the listed
-// tokens that difference would be rounding noise, and log s and t / s with it.
+// the listed elements. The row is summed without the listed elements, which join it in fp64: s is never
+// 1 - sum q, which for a student that is sure of the listed tokens would be rounding noise, and log s, t / s
+// and -log q with it (a loss of 1e-4 was off by 4e-4 where an fp32 sum held the listed elements too).
 #pragma once
 #include "list_rows.h"
 
@@ -225,21 +226,18 @@ struct ListTerms {
   float centre, l2;    // q = 2^((x - centre) cT - l2)
 };
 
-// One wave. `sum`: the student's softmax sum, without the listed elements for the kinds with a tail, of
-// the whole row for the other. fp64: a few hundred operations of one wave per row.
+// One wave. `sum`: the student's softmax sum without the listed elements. fp64: a few hundred operations of
+// one wave per row.
 __device__ __forceinline__ ListTerms list_terms(const ListEntries& e, const TeacherTerms& teacher, const StudentTerms& student,
                                                 const RowTotals& sum, int kind, double temperature, int64_t vocab) {
   ListTerms r;
   const double inv_t = 1.0 / temperature;
   const bool tail = kind != ORLHF_DISTILL_FORWARD;
   const bool some = sum.sT > 0.0 || sum.sT != sum.sT;  // anything of weight outside the list
-  double base = some ? sum.base_t : -INFINITY, total = sum.sT;
-  if (tail) {
-    const double rest_base = base;
-    if (student.top > base) base = student.top;
-    const double listed = student.sum * (student.top == base ? 1.0 : exp(student.top - base));
-    total = (some ? sum.sT * (rest_base == base ? 1.0 : exp(rest_base - base)) : 0.0) + (teacher.n_on > 0 ? listed : 0.0);
-  }
+  const double rest_base = some ? sum.base_t : -INFINITY, base = student.top > rest_base ? student.top : rest_base;
+  const double listed = student.sum * (student.top == base ? 1.0 : exp(student.top - base));
+  const double total =
+      (some ? sum.sT * (rest_base == base ? 1.0 : exp(rest_base - base)) : 0.0) + (teacher.n_on > 0 ? listed : 0.0);
   const double log_total = sum.nan ? (double)NAN : log(total);
   double lq[2], q[2], part[2];
 #pragma unroll

@@ -369,3 +369,53 @@ def test_teacher_targets_to_aggregated_student_loss(cuda):
     rel = 2 * (3 + 3 * 12 * 1.45 + 24) * U
     assert ((kl - kl2).abs() <= 4 * rel * (1 + kl.abs())).all()
     assert ((grad - grad2).abs() <= 8 * rel * grad.abs() + 4 * rel * weights.unsqueeze(-1)).all()
+
+
+def _sum_error(x, temperature):
+    """Relative error of the sum outside the list: one rounding per term of an accumulator (two in each of
+    256 lanes: V / 512), the rounding of the exponents (X = max |x|), and the additions that join them."""
+    big = x[x.abs() < 1e30].abs().max().item()
+    return (x.numel() / 512 + 3 * big * math.log2(math.e) / temperature + 24) * U
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("vocab,dtype", [(2100, "fp32"), (33000, "bf16"), (80011, "fp16")])
+@pytest.mark.parametrize("rows", [5, 300, 530])
+def test_small_divergences_keep_their_digits(cuda, form, vocab, dtype, rows):
+    """Teachers that nearly agree and students that are sure of the listed tokens, where the loss is a
+    difference of much larger terms. Only R, the sum outside the list, is an fp32 sum (relative error d):
+    the loss moves by dL/dlog R times d, that is ((P + t) s - t) d, s d and s (log(s / t) - L) d, by terms of
+    d^2, and is rounded once (1e-12: the fp64 terms that cancel)."""
+    from openrlhf_amd.models.utils import distill_kl_from_logits, fused_distill_kl_fwd_bwd
+
+    g = torch.Generator().manual_seed(vocab + rows)
+    k, temperature = 6, 0.9
+    x = torch.randn(rows, vocab, generator=g)
+    listed = torch.stack([torch.randperm(vocab, generator=g)[:k] for _ in range(rows)])
+    x.scatter_add_(1, listed, torch.rand(rows, k, generator=g) * 3 + math.log(vocab) + torch.arange(rows).view(-1, 1) % 4 * 3.0)
+    x = x.to(TYPES[dtype])
+    near = x.double() + torch.randn(rows, vocab, generator=g).double() * (0.02 * (torch.arange(rows) % 3)).view(-1, 1)
+    lps = torch.log_softmax(near / temperature, -1).gather(1, listed).float()
+    view, idc, lpc = x.cuda(), listed.cuda(), lps.cuda()
+    outs = [distill_kl_from_logits(view, idc, lpc, temperature, *form),
+            fused_distill_kl_fwd_bwd(view, idc, lpc, torch.ones(rows, device="cuda"), temperature, *form, inplace=False)[0]]
+    few = range(rows) if rows < 20 else list(range(0, 12)) + [rows - 2, rows - 1]
+    small = 0
+    for r, (want, _, x64) in zip(few, _reference(view, listed, lps, temperature, form, few)):
+        d = _sum_error(x64, temperature)
+        q = torch.log_softmax(x64 / temperature, -1).exp()
+        inside = torch.zeros(vocab, dtype=torch.bool)
+        inside[listed[r]] = True
+        s, p = q[~inside].sum().item(), lps[r].double().exp()
+        if form == ("forward", False):
+            first = s
+        elif form == ("forward", True):
+            t = max(0.0, 1.0 - p.sum().item())
+            first = abs((p.sum().item() + t) * s - t)
+        else:
+            t = max(2.0 ** -24, 1.0 - p.sum().item())
+            first = abs(s * (math.log(s / t) - want))
+        small += abs(want) < 1e-3
+        for out in outs:
+            assert abs(out[r].item() - want) <= first * d + 4 * d * d + 2 * U * abs(want) + 1e-12, (r, out[r].item(), want, s)
+    assert small > 0
