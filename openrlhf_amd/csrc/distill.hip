@@ -216,7 +216,7 @@ extern "C" int orlhf_distill_kl_fwd(const void* logits, int dtype, int64_t n_row
                   (long long)workspace_bytes);
   ORLHF_CHECK_ARG(((uintptr_t)tickets & 3u) == 0, "distill_kl_fwd: tickets not 4-byte aligned");
   const DistillArgs a = {(const char*)logits, n_rows, vocab, row_stride * esize,
-                         {teacher_ids, teacher_logprob, (int)k, 1.0 / teacher_temperature},
+                         {teacher_ids, teacher_logprob, (int)k, 1.0 / teacher_temperature, kind == ORLHF_DISTILL_FORWARD},
                          temperature, kind, loss, row_stats, list_grad, list_at, row_mask,
                          list_split(n_rows, vocab, (int)esize), (uint64_t*)workspace, tickets};
   hipStream_t s = (hipStream_t)stream;

@@ -479,7 +479,7 @@ extern "C" int orlhf_distill_kl_fwd_bwd(const void* logits, void* grad_logits, i
     if (hipDeviceGetAttribute(&v, hipDeviceAttributeMultiprocessorCount, device) == hipSuccess && v > 0) n_cu = v;
   }
   OneArgs a = {(const char*)logits, (char*)grad_logits, n_rows, vocab, row_stride * esize, grad_row_stride * esize,
-               {teacher_ids, teacher_logprob, (int)k, 1.0 / teacher_temperature},
+               {teacher_ids, teacher_logprob, (int)k, 1.0 / teacher_temperature, kind == ORLHF_DISTILL_FORWARD},
                temperature, kind, weight, loss, row_mask, (uint32_t)(ListMap<ORLHF_BF16>::bytes(vocab) / 4)};
   const unsigned blocks = (unsigned)(n_rows < n_cu ? n_rows : n_cu);  // a workgroup takes a CU's register file
   hipStream_t s = (hipStream_t)stream;

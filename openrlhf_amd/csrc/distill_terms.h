@@ -22,13 +22,22 @@ constexpr int64_t kMaxDistillVocab = 520192;  // a bit per element in 64 KiB of 
 constexpr double kTinyTail = 5.9604644775390625e-08;  // 2^-24
 constexpr double kLogTinyRest = -87.33654475055310898657;  // log 2^-126: the student's tail mass is taken to be at least that
 
+__device__ __forceinline__ double wave_max(double v) {
+#pragma unroll
+  for (int o = kWave / 2; o > 0; o >>= 1) {
+    const double other = __shfl_xor(v, o, kWave);
+    v = other > v ? other : v;
+  }
+  return v;
+}
+
 // Teacher's list of one row and the student's logits there, held by one wave: entry lane + 64 i. An entry
 // with a negative id or a log-prob of -inf is absent, one past the vocabulary is absent and makes the
 // loss NaN, an id that comes twice counts once with the sum of its probabilities.
 struct ListEntries {
   int id[2];     // -1: absent
   float x[2];    // the student's logit
-  double lp[2];  // the teacher's log-prob
+  double lp[2];  // the teacher's log-prob; where the list is renormalised relative to its largest value
   bool bad;
 };
 
@@ -37,6 +46,7 @@ struct ListSource {
   const float* teacher;
   int k;
   double inv_teacher_t;
+  bool renormalise;  // the values are to go through a softmax: logits of any size
 };
 
 // The row's list as it stands in memory.
@@ -70,6 +80,11 @@ __device__ __forceinline__ ListEntries settle_list(const RawList& raw, const Lis
     e.x[i] = e.id[i] >= 0 ? E::load1(row + (int64_t)e.id[i] * E::kSize) : 0.0f;
   }
   e.bad = __ballot(e.bad) != 0ull;
+  if (src.renormalise) {  // the largest value comes off before anything is exponentiated
+    const double a = e.id[0] >= 0 ? e.lp[0] : -INFINITY, b = e.id[1] >= 0 ? e.lp[1] : -INFINITY;
+    const double top = wave_max(a > b ? a : b);
+    e.lp[0] -= top, e.lp[1] -= top;
+  }
   return e;
 }
 
@@ -86,28 +101,37 @@ __device__ __forceinline__ bool list_repeats(const ListEntries& e, int k) {
   return __ballot(again) != 0ull;
 }
 
-// Adds the probabilities of an id's later entries to its first, in their order, and drops them.
+// Adds the probabilities of an id's later entries to its first, in their order, and drops them. Relative to the
+// largest of them: the values may be logits of any size.
 __device__ __forceinline__ void join_repeats(ListEntries& e, int k) {
   const int lane = threadIdx.x & (kWave - 1);
-  double sum[2] = {exp(e.lp[0]), exp(e.lp[1])};
-  bool more[2] = {false, false}, again[2] = {false, false};
+  auto each_twin = [&](auto&& f) {
 #pragma unroll 1
-  for (int j = 0; j < k; ++j) {
-    const bool second = j >= kWave;
-    const int other = __shfl(second ? e.id[1] : e.id[0], j & (kWave - 1), kWave);
-    const double lp = __shfl(second ? e.lp[1] : e.lp[0], j & (kWave - 1), kWave);
+    for (int j = 0; j < k; ++j) {
+      const bool second = j >= kWave;
+      const int other = __shfl(second ? e.id[1] : e.id[0], j & (kWave - 1), kWave);
+      const double lp = __shfl(second ? e.lp[1] : e.lp[0], j & (kWave - 1), kWave);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int at = lane + i * kWave;
-      if (other >= 0 && e.id[i] == other && at != j) {
-        if (at < j) sum[i] += exp(lp), more[i] = true;
-        if (at > j) again[i] = true;
+      for (int i = 0; i < 2; ++i) {
+        const int at = lane + i * kWave;
+        if (other >= 0 && e.id[i] == other && at != j) f(i, at < j, lp);
       }
     }
-  }
+  };
+  double top[2] = {e.lp[0], e.lp[1]};
+  bool more[2] = {false, false}, again[2] = {false, false};
+  each_twin([&](int i, bool later, double lp) {
+    if (later) more[i] = true;
+    if (!later) again[i] = true;
+    top[i] = lp > top[i] ? lp : top[i];
+  });
+  double sum[2] = {exp(e.lp[0] - top[0]), exp(e.lp[1] - top[1])};
+  each_twin([&](int i, bool later, double lp) {
+    if (later) sum[i] += exp(lp - top[i]);
+  });
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    if (more[i]) e.lp[i] = log(sum[i]);
+    if (more[i]) e.lp[i] = top[i] + log(sum[i]);
     if (again[i]) e.id[i] = -1;
   }
 }
@@ -172,19 +196,10 @@ struct WithoutListed {
   }
 };
 
-__device__ __forceinline__ double wave_max(double v) {
-#pragma unroll
-  for (int o = kWave / 2; o > 0; o >>= 1) {
-    const double other = __shfl_xor(v, o, kWave);
-    v = other > v ? other : v;
-  }
-  return v;
-}
-
 // What the loss takes from the teacher alone and from the student's listed logits alone: each one wave's
 // work that does not wait for the row.
 struct TeacherTerms {
-  double p[2];  // of this lane's entries, 0 where absent
+  double p[2];  // of this lane's entries, 0 where absent; for the kind without a tail up to the factor 1 / mass
   double mass, t, log_t, log_mass;
   int n_on;
 };

@@ -48,10 +48,13 @@ def distill_kl_row(logits, ids, teacher, temperature=1.0, teacher_temperature=1.
     zero = logits.sum() * 0.0
     if not listed:
         return zero
-    log_p = {i: torch.logsumexp(torch.tensor(v, dtype=torch.float64), 0).item() for i, v in listed.items()}
+    joined = lambda off: {i: torch.logsumexp(torch.tensor(v, dtype=torch.float64) - off, 0).item() for i, v in listed.items()}  # noqa: E731
+    if kl == "forward" and not tail:  # a softmax: the values may be logits of any size, their largest comes off first
+        log_p = joined(max(max(v) for v in listed.values()))
+        log_w = torch.log_softmax(torch.tensor(list(log_p.values()), dtype=torch.float64), 0).tolist()
+        return zero + sum(math.exp(v) * (v - log_q[i]) for i, v in zip(log_p, log_w))
+    log_p = joined(0.0)
     mass = math.fsum(math.exp(v) for v in log_p.values())
-    if kl == "forward" and not tail:
-        return zero + sum(math.exp(v) / mass * (v - math.log(mass) - log_q[i]) for i, v in log_p.items())
     outside = torch.ones_like(logits, dtype=torch.bool)
     outside[list(log_p)] = False
     s = log_q.exp()[outside].sum().clamp(min=2.0 ** -126)

@@ -419,3 +419,45 @@ def test_small_divergences_keep_their_digits(cuda, form, vocab, dtype, rows):
         for out in outs:
             assert abs(out[r].item() - want) <= first * d + 4 * d * d + 2 * U * abs(want) + 1e-12, (r, out[r].item(), want, s)
     assert small > 0
+
+
+@pytest.mark.parametrize("teacher_temperature,shift,scale", [
+    (1.0, 1000.0, 3.0),    # logits with a constant offset
+    (1.0, -1000.0, 3.0),
+    (0.05, 40.0, 3.0),     # ordinary logits at a low temperature
+    (0.01, -30.0, 1.0),
+    (1.0, 0.0, 300.0),     # one token far above the others
+    (1.0, -720.0, 2.0),    # probabilities that would be subnormal
+    (2.0, 3.0e38, 0.0),    # at the end of fp32
+])
+@pytest.mark.parametrize("n", [4, 300])
+def test_teacher_logits_of_any_size(cuda, teacher_temperature, shift, scale, n):
+    """tail=False takes the teacher's logits as they come: w = softmax(values / teacher_temperature), with
+    repeated, absent and lowest-value entries among them."""
+    from openrlhf_amd.models.utils import distill_kl_from_logits, fused_distill_kl_fwd_bwd
+
+    view, ids, _, g = _case(n, 5003, 12, "fp32", 31)
+    raw = torch.randn(n, 12, generator=g) * scale + shift
+    ids[1, 7] = ids[1, 2]
+    ids[2, 3] = ids[2, 9] = ids[2, 0]
+    raw[2, 0] = raw[2].max()
+    ids[3, 5], raw[3, 6] = -1, -math.inf
+    raw[3, 8] = torch.finfo(torch.float32).min
+    weight = torch.rand(n, generator=g) + 0.2
+    leaf = view.detach().requires_grad_(True)
+    idc, rawc = ids.cuda(), raw.cuda()
+    loss = distill_kl_from_logits(leaf, idc, rawc, 1.2, tail=False, teacher_temperature=teacher_temperature)
+    (grad,) = torch.autograd.grad([loss], [leaf], [weight.cuda()])
+    rows = range(4)
+    want = _reference(view, ids, raw, 1.2, ("forward", False), rows, teacher_temperature)
+    for r, (value, d, x) in zip(rows, want):
+        rel = 2 * _sum_error(x, 1.2)
+        # w: fp64 quotients of fp32 inputs; log w / q of terms up to max |log w| + max |log q|
+        lq = torch.log_softmax(x / 1.2, -1)
+        size = 2 * U * (abs(value) + 1)
+        bound = (lq.exp() * (rel + 4 * U * (lq.abs() + 4)) + 4 * U * (d.abs() + lq.exp())) / 1.2
+        for l, gr in ((loss, grad), fused_distill_kl_fwd_bwd(view, idc, rawc, weight.cuda(), 1.2, tail=False, inplace=False,
+                                                             teacher_temperature=teacher_temperature)):
+            assert abs(l[r].item() - value) <= rel + size, (r, l[r].item(), value)
+            w = weight[r].item()
+            assert ((gr[r].double().cpu() - w * d).abs() <= w * bound + 1e-37).all(), r
