@@ -189,8 +189,10 @@ int orlhf_top_logprobs_fwd(const void* logits, int dtype, int64_t n_rows, int64_
  *   sum_k g_top[i,k] * (1[j==top_ids[i,k]] - softmax(logits/temperature)[i,j]) / temperature
  * `grad_logits` may alias `logits` (same row stride). g_logprob, g_entropy float [n_rows] and
  * g_top_logprob float [n_rows, k]: each may be NULL (zero), not all. The ids of a row have to be
- * distinct, as the forward gives them; ids outside [0, vocab) get no one-hot term. Rows whose
- * upstream gradients are all 0, or with row_mask 0, are written as zeros without being read.
+ * distinct, as the forward gives them; ids outside [0, vocab) get no one-hot term. The g_logprob of a
+ * row with label -100 is taken as 0 (its log-prob is a constant); that of another label outside the
+ * vocabulary, whose log-prob is NaN, has no one-hot term. Rows whose upstream gradients are all 0, or
+ * with row_mask 0, are written as zeros without being read.
  */
 int orlhf_top_logprobs_bwd(const void* logits, void* grad_logits, int dtype, int64_t n_rows,
                            int64_t vocab, int64_t row_stride, int64_t grad_row_stride,

@@ -319,7 +319,7 @@ __device__ __forceinline__ void write_row(const TopArgs& a, int64_t row_i, const
   }
   if (tid == 0) {
     if (a.logprob != nullptr)
-      a.logprob[row_i] = label >= 0 && label < a.vocab ? logprob_of(x_label, a.temperature, softmax) : (label == -100 ? 0.0f : NAN);
+      a.logprob[row_i] = label >= 0 && label < a.vocab ? logprob_of(x_label, a.temperature, softmax) : (label == kIgnoredLabel ? 0.0f : NAN);
     if (ModeTraits<MODE>::kPlainSet && a.entropy != nullptr) a.entropy[row_i] = (float)softmax.entropy;
     if (a.row_stats != nullptr) *(f32x4*)(a.row_stats + row_i * 4) = f32x4{softmax.centre, softmax.l2_t, softmax.l2_1, softmax.ex};
   }
@@ -502,7 +502,8 @@ __global__ __launch_bounds__(kBlock) void top_logprobs_bwd_kernel(TopBwdArgs a) 
 #pragma unroll
   for (int i = 0; i < kWavesPerBlock; ++i) sum_top += lds[i];
   __syncthreads();
-  const float glp = a.g_logprob != nullptr ? a.g_logprob[row_i] : 0.0f;
+  const int64_t label = a.g_logprob != nullptr ? a.labels[row_i] : -1;
+  const float glp = a.g_logprob != nullptr && label != kIgnoredLabel ? a.g_logprob[row_i] : 0.0f;  // ignored: a constant
   const float gh = MODE != kBwdLp ? a.g_entropy[row_i] : 0.0f;
   if (skipped || (glp == 0.0f && gh == 0.0f && !top_on)) {
     zero_row<DT>(out_row, g);
@@ -519,7 +520,6 @@ __global__ __launch_bounds__(kBlock) void top_logprobs_bwd_kernel(TopBwdArgs a) 
   fn.onehot = (float)((double)glp * inv_t);
   fn.gh = gh;
   fn.k1 = gh * st[3] + (MODE == kBwdBothT1 ? fn.a_all : 0.0f);
-  const int64_t label = a.g_logprob != nullptr ? a.labels[row_i] : -1;
   fn.set_label(label >= 0 && label < a.vocab ? label - (int64_t)seg.first : -1, seg.len, g, E::kPerVec);
   const bool patch = mine && id >= 0 && id < seg.len;
   float val = 0.0f;

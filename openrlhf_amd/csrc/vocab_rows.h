@@ -16,6 +16,8 @@
 
 namespace orlhf {
 
+constexpr int64_t kIgnoredLabel = -100;  // its log-prob is the constant 0, without a gradient
+
 // ---------------------------------------------------------------- element traits
 template <int DT>
 struct Elt;

@@ -321,7 +321,8 @@ def top_logprobs_from_logits(
     The alternatives are the k largest logits, descending, equal logits by ascending id (a NaN ranks
     before everything); their log-probs, like the label's, are those of ``logits / temperature``, the
     entropy is that of the unscaled logits. ``labels=None`` leaves the log-probs out (None is
-    returned), ``return_entropy=False`` the entropy. ``1 <= k <= 128``.
+    returned), ``return_entropy=False`` the entropy; a label of -100 has log-prob 0 and no gradient.
+    ``1 <= k <= 128``.
 
     Differentiable in the three float outputs (the choice of the tokens is taken as given).
     ``inplace_backward`` and ``row_mask`` as in ``logprobs_and_entropy_from_logits``; a position with

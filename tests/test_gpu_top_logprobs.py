@@ -359,3 +359,29 @@ def test_repeats_other_stream_and_replayed_graph_give_the_same_bits(cuda, rows):
         torch.cuda.synchronize()
         for a, b in zip(captured, expect):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("vocab", [4099, 40009])
+@pytest.mark.parametrize("temperature", [1.0, 0.8])
+def test_an_ignored_label_has_no_gradient(cuda, vocab, temperature):
+    """Label -100: the log-prob is the constant 0, so its upstream gradient reaches no logit; the entropy's
+    and the alternatives' do. The same row with a label inside and upstream gradient 0 gives the same bits."""
+    from openrlhf_amd.models.utils import top_logprobs_from_logits
+
+    view, labels, g = _logits(6, vocab, "fp32", 12)
+    labels[1] = labels[4] = -100
+    at = labels == -100
+    g_lp, g_ent, g_top = torch.randn(6, generator=g) + 3.0, torch.randn(6, generator=g), torch.randn(6, 5, generator=g)
+    zeroed, inside = g_lp.masked_fill(at, 0.0), labels.masked_fill(at, 7)
+    for use in ((1, 0, 0), (1, 1, 0), (1, 0, 1), (1, 1, 1)):
+        grads = []
+        for lab, glp in ((labels, g_lp), (inside, zeroed)):
+            leaf = view.detach().requires_grad_(True)
+            lp, ent, top, ids = top_logprobs_from_logits(leaf, lab.cuda(), 5, temperature, return_entropy=bool(use[1]))
+            pairs = [(o, q.cuda()) for o, q, on in zip((lp, ent, top), (glp, g_ent, g_top), use) if on]
+            grads.append(torch.autograd.grad([p[0] for p in pairs], [leaf], [p[1] for p in pairs])[0])
+            assert ((lp == 0) == (lab == -100).cuda()).all()
+        assert torch.equal(grads[0], grads[1])
+        if not use[1] and not use[2]:
+            assert (grads[0][at.cuda()] == 0).all() and (grads[0][~at.cuda()] != 0).any(1).all()
+    _check_grad(view, grads[0], inside, ids.cpu(), zeroed, g_ent, g_top, temperature, range(6))
