@@ -148,8 +148,10 @@ int orlhf_logprob_entropy_fwd_split(const void* logits, int dtype, int64_t n_row
  *             + g_entropy[i] * softmax(x)[i,j] * (E[x] - x[i,j])
  * `grad_logits` may alias `logits` (in-place: each 16-byte chunk is read, then overwritten by the
  * same lane). Replaces torch autograd through openrlhf/models/utils.py:139-163 and :182-186.
- * g_logprob / g_entropy: float [n_rows] or NULL (treated as 0). Rows whose upstream gradients
- * are both exactly 0, and rows with row_mask 0 (same array as in the forward, or NULL), are
+ * g_logprob / g_entropy: float [n_rows] or NULL (treated as 0). The g_logprob of a row with label
+ * -100 is taken as 0 (its log-prob is a constant; the one-pass and lm-head forms below do the same);
+ * that of another label outside [0, vocab), whose log-prob is NaN, has no one-hot term. Rows whose
+ * upstream gradients are both exactly 0, and rows with row_mask 0 (same array as in the forward, or NULL), are
  * written as zeros without reading their logits.
  */
 int orlhf_logprob_entropy_bwd(const void* logits, void* grad_logits, int dtype, int64_t n_rows,

@@ -304,7 +304,7 @@ __global__ __launch_bounds__(kCombineBlock) void lmhead_combine_kernel(const flo
     if (label >= 0 && label < vocab)
       lp = (float)((double)x_label[tok] * inv_t - lseT);
     else
-      lp = (label == -100) ? 0.0f : NAN;
+      lp = (label == kIgnoredLabel) ? 0.0f : NAN;
     logprob[tok] = lp;
   }
   if (entropy != nullptr) entropy[tok] = (float)(lse1 - ex);
@@ -318,8 +318,9 @@ __global__ __launch_bounds__(kCombineBlock) void lmhead_combine_kernel(const flo
 // a token's P does not depend on which of the two produced it.
 template <int MODE>
 __device__ __forceinline__ GradFn<MODE> token_grad_fn(const float* __restrict__ row_stats, const float* __restrict__ g_logprob,
-                                                     const float* __restrict__ g_entropy, int64_t tok, double inv_t, bool& dead) {
-  const float glp = g_logprob != nullptr ? g_logprob[tok] : 0.0f;
+                                                     const float* __restrict__ g_entropy, int64_t tok, int64_t label,
+                                                     double inv_t, bool& dead) {
+  const float glp = g_logprob != nullptr && label != kIgnoredLabel ? g_logprob[tok] : 0.0f;  // ignored: a constant
   const float gh = g_entropy != nullptr ? g_entropy[tok] : 0.0f;
   const f32x4 st = *(const f32x4*)(row_stats + tok * 4);
   GradFn<MODE> fn;
@@ -366,8 +367,9 @@ __global__ __launch_bounds__(mm::kThreads, 1) void lmhead_bwd_p_kernel(Operand w
     const int64_t tok = (int64_t)tb * 256 + mm::acc_col(wn, nt, lane);
     if (tok >= n_tokens) continue;
     bool dead;
-    const GradFn<MODE> fn = token_grad_fn<MODE>(row_stats, g_logprob, g_entropy, tok, inv_t, dead);
-    const int64_t d = (labels != nullptr ? labels[tok] : -1) - vbase;
+    const int64_t label = labels != nullptr ? labels[tok] : -1;
+    const GradFn<MODE> fn = token_grad_fn<MODE>(row_stats, g_logprob, g_entropy, tok, label, inv_t, dead);
+    const int64_t d = label - vbase;
     const int lab_rel = (d >= 0 && d < 128) ? (int)d : -1;
     uint16_t* out = p_chunk + tok * ldp + ((int64_t)ct * 256 + wm * 128 + 4 * (lane >> 5));
 #pragma unroll
@@ -408,8 +410,8 @@ __global__ __launch_bounds__(kBlock) void lmhead_p_inplace_kernel(uint16_t* __re
     const int64_t tok = item / stretches, c0 = (item - tok * stretches) * kInplaceCols;
     const int64_t c1 = c0 + kInplaceCols < kept_cols ? c0 + kInplaceCols : kept_cols;
     bool dead;
-    const GradFn<MODE> fn = token_grad_fn<MODE>(row_stats, g_logprob, g_entropy, tok, 1.0 / temperature, dead);
     const int64_t label = labels != nullptr ? labels[tok] : -1;
+    const GradFn<MODE> fn = token_grad_fn<MODE>(row_stats, g_logprob, g_entropy, tok, label, 1.0 / temperature, dead);
     char* row = (char*)(kept + tok * kept_ld);
     for (int64_t c = c0 + (int64_t)threadIdx.x * 8; c < c1; c += kBlock * 8) {  // kept_cols is a multiple of 8
       float x[8];

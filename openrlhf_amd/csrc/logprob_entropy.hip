@@ -118,7 +118,7 @@ __device__ __forceinline__ void merge_row(int64_t row_i, int64_t vocab, const in
     if (label >= 0 && label < vocab) {
       lp = (float)((double)x_label / temperature - lse_t);
     } else {
-      lp = (label == -100) ? 0.0f : NAN;
+      lp = (label == kIgnoredLabel) ? 0.0f : NAN;
     }
     logprob[row_i] = lp;
   }
@@ -329,7 +329,7 @@ __global__ __launch_bounds__(kBlock) void logprob_entropy_fwd_kernel(
         if (label >= 0 && label < vocab) {
           lp = (float)((double)x_label / temperature - lse_t);
         } else {
-          lp = (label == -100) ? 0.0f : NAN;
+          lp = (label == kIgnoredLabel) ? 0.0f : NAN;
         }
         logprob[row_i] = lp;
       }
@@ -383,7 +383,8 @@ __global__ __launch_bounds__(kBlock) void logprob_entropy_bwd_kernel(
     // (the host guarantees both have the same 16-byte phase unless scalar_only is set)
     const RowGeom g = row_geom<DT>(row, item.len, scalar_only != 0);
 
-    const float glp = (MODE != kBwdEnt) ? g_logprob[row_i] : 0.0f;
+    const int64_t label = (MODE != kBwdEnt) ? labels[row_i] : -1;
+    const float glp = (MODE != kBwdEnt && label != kIgnoredLabel) ? g_logprob[row_i] : 0.0f;  // ignored: a constant
     const float gh = (MODE != kBwdLp) ? g_entropy[row_i] : 0.0f;
     const bool skipped = row_mask != nullptr && row_mask[row_i] == 0;  // forward gave constants
     if (skipped || (glp == 0.0f && gh == 0.0f)) {
@@ -401,7 +402,6 @@ __global__ __launch_bounds__(kBlock) void logprob_entropy_bwd_kernel(
     fn.gh = gh;
     fn.k1 = gh * st[2] - (MODE == kBwdBothT1 ? glp : 0.0f);
     // the label relative to this segment; outside it (or outside the vocabulary) no element gets the one-hot term
-    const int64_t label = (MODE != kBwdEnt) ? labels[row_i] : -1;
     fn.set_label((label >= 0 && label < vocab) ? label - (int64_t)item.first : -1, item.len, g, Elt<DT>::kPerVec);
     traverse_row<DT, true>(row, out_row, g, fn);
   }

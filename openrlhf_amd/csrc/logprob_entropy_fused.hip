@@ -293,12 +293,13 @@ __global__ __launch_bounds__(kFusedBlock) void logprob_entropy_fused_pipe_kernel
         ex = NAN;
       }
       const int64_t label = (MODE != kEntOnly) ? labels[row_i] : -1;
+      const bool ignored = label == kIgnoredLabel;
       float lp = 0.0f;
       if (MODE != kEntOnly) {
         if (label >= 0 && label < vocab)
           lp = (float)((double)E::load1(row + label * E::kSize) * inv_t - lse_t);
         else
-          lp = (label == -100) ? 0.0f : NAN;
+          lp = ignored ? 0.0f : NAN;
         if (logprob != nullptr) logprob[row_i] = lp;
       }
       if (MT::kPlainSet && entropy != nullptr) entropy[row_i] = (float)(lse_1 - ex);
@@ -323,6 +324,7 @@ __global__ __launch_bounds__(kFusedBlock) void logprob_entropy_fused_pipe_kernel
         glp = (MODE != kEntOnly && w_logprob != nullptr) ? w_logprob[row_i] : 0.0f;
         gh = (MT::kPlainSet && w_entropy != nullptr) ? w_entropy[row_i] : 0.0f;
       }
+      if (ignored) glp = 0.0f;  // the log-prob is a constant
       lds_bcast[0] = -(float)(lse_t * 1.4426950408889634);
       lds_bcast[1] = -(float)(lse_1 * 1.4426950408889634);
       lds_bcast[2] = -(float)((double)glp * inv_t);

@@ -169,7 +169,8 @@ def logprobs_and_entropy_from_logits(
     ``inplace_backward=True`` writes d(loss)/d(logits) over the logits storage in backward
     instead of allocating a second [N, V] tensor; the logits are unusable afterwards.
     ``row_mask`` (same shape as ``labels``): positions with 0 are skipped, their outputs are 0
-    and their logits get zero gradient without being read (prompt and padding positions).
+    and their logits get zero gradient without being read (prompt and padding positions). A label of
+    -100 has log-prob 0 and no gradient (``ignore_index`` of a cross entropy).
     """
     return _LogprobEntropy.apply(logits, labels, temperature, True, True, inplace_backward, row_mask)
 

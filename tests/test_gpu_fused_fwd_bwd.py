@@ -258,3 +258,68 @@ def test_fused_many_rows_per_workgroup(cuda, rows, vocab, dtype, std, temperatur
     else:
         eps = 2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -11
         assert (err <= eps * ref.abs() + 1e-6).all(), err.max().item()
+
+
+# ------------------------------------------------------------------ ignored labels (-100)
+@pytest.mark.parametrize("rows,vocab,dtype", [(5, 70001, torch.bfloat16), (300, 4099, torch.float32), (300, 151936, torch.bfloat16)])
+@pytest.mark.parametrize("temperature", [1.0, 0.7])
+@pytest.mark.parametrize("entropy", [False, True])
+def test_an_ignored_label_has_no_gradient(cuda, rows, vocab, dtype, temperature, entropy):
+    """Label -100 makes the log-prob the constant 0: its upstream gradient reaches no logit (cross entropy with
+    ignore_index), in the backward and in the one-pass form, whose entropy part is as for any other label.
+    Checked as the bits of the same call with a label inside and an upstream gradient of 0."""
+    from openrlhf_amd.models.utils import fused_logprob_entropy_fwd_bwd, logprobs_and_entropy_from_logits, log_probs_from_logits
+
+    g = torch.Generator().manual_seed(rows + vocab)
+    x = (torch.randn(rows, vocab, generator=g) * 2).to(dtype).to(cuda)
+    labels = torch.randint(0, vocab, (rows,), generator=g)
+    at = torch.arange(rows) % 3 == 1
+    ignored = labels.masked_fill(at, -100).to(cuda)
+    g_lp, g_ent = torch.randn(rows, generator=g) + 3.0, torch.randn(rows, generator=g).to(cuda)
+    zeroed, g_lp = g_lp.masked_fill(at, 0.0).to(cuda), g_lp.to(cuda)
+    labels, at = labels.to(cuda), at.to(cuda)
+    grads, fused = [], []
+    for lab, up in ((ignored, g_lp), (labels, zeroed)):
+        leaf = x.detach().requires_grad_(True)
+        if entropy:
+            lp, ent = logprobs_and_entropy_from_logits(leaf, lab, temperature)
+            grads.append(torch.autograd.grad([lp, ent], [leaf], [up, g_ent])[0])
+        else:
+            lp = log_probs_from_logits(leaf, lab, temperature)
+            grads.append(torch.autograd.grad([lp], [leaf], [up])[0])
+        assert ((lp == 0) == (lab == -100)).all()
+        fused.append(fused_logprob_entropy_fwd_bwd(x.clone(), lab, up, g_ent if entropy else None, temperature)[2])
+    for a, b in (grads, fused):
+        assert torch.equal(a, b)
+        if not entropy:
+            assert (a[at] == 0).all() and (a[~at] != 0).any(1).all()
+
+
+def test_an_ignored_label_has_no_gradient_in_the_step_form(cuda):
+    """The form that derives its upstream gradients from the log-prob: an ignored label's is the constant 0, so
+    only the entropy term of such a row is left, the bits of a row with a label inside and no policy weight."""
+    from ctypes import byref
+
+    from openrlhf_amd import _lib
+
+    rows, vocab = 20, 5000
+    g = torch.Generator().manual_seed(3)
+    x = torch.randn(rows, vocab, generator=g).to(cuda)
+    labels = torch.randint(0, vocab, (rows,), generator=g)
+    at = torch.arange(rows) % 3 == 0
+    one = lambda: torch.rand(rows, generator=g).to(cuda)  # noqa: E731
+    old, adv, token = -one() * 8, one() + 0.5, one()
+    policy = one() + 0.1
+    grads = []
+    for lab, coef in ((labels.masked_fill(at, -100), policy), (labels, policy.masked_fill(at.to(cuda), 0.0))):
+        t = _lib.StepTerms()
+        t.old_log_probs, t.advantages, t.policy_coef, t.token_coef = (v.data_ptr() for v in (old, adv, coef, token))
+        t.clip_eps_low = t.clip_eps_high = 1e30
+        t.is_correction, t.kl_estimator, t.kl_coef, t.entropy_coef = _lib.IS_NONE, _lib.KL_K1, 0.0, 0.01
+        grad, lp, ent = torch.empty_like(x), torch.empty(rows, device=cuda), torch.empty(rows, device=cuda)
+        ld = lab.to(cuda)
+        _lib.call("orlhf_policy_step_fwd_bwd", x.data_ptr(), grad.data_ptr(), _lib.F32, rows, vocab, vocab, vocab, ld.data_ptr(),
+                  1.0, byref(t), lp.data_ptr(), ent.data_ptr(), None, _lib.stream_of(cuda))
+        grads.append(grad)
+        assert ((lp == 0) == (ld == -100)).all()
+    assert torch.equal(grads[0], grads[1]) and (grads[0] != 0).any(1).all()

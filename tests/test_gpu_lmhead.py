@@ -321,3 +321,30 @@ def test_lmhead_outputs_at_any_stride_and_alignment_hold_the_same_bits(cuda):
         other = run(kept_ld, offset, pad)
         for a, b in zip(aligned, other):
             assert torch.equal(a.view(torch.int16) if a.dtype == torch.bfloat16 else a, b.view(torch.int16) if b.dtype == torch.bfloat16 else b), (kept_ld, offset, pad)
+
+
+@pytest.mark.parametrize("temperature", [1.0, 0.8])
+@pytest.mark.parametrize("keep_mib", [None, 1])
+def test_lmhead_ignored_label_has_no_gradient(cuda, temperature, keep_mib):
+    """Label -100 makes the log-prob the constant 0: only the entropy's upstream gradient of such a position
+    reaches the hidden states and the weight, the bits of a label inside with an upstream gradient of 0."""
+    from openrlhf_amd.models.utils import lm_head_logprobs_and_entropy
+
+    n, hdim, vocab = 70, 64, 3000
+    g = torch.Generator().manual_seed(9)
+    hidden = torch.randn(n, hdim, generator=g).to(torch.bfloat16).to(cuda)
+    weight = (torch.randn(vocab, hdim, generator=g) * 0.3).to(torch.bfloat16).to(cuda)
+    labels = torch.randint(0, vocab, (n,), generator=g)
+    at = torch.arange(n) % 4 == 2
+    g_lp, g_ent = torch.randn(n, generator=g) + 3.0, torch.randn(n, generator=g)
+    grads = []
+    for with_entropy in (False, True):
+        for lab, up in ((labels.masked_fill(at, -100), g_lp), (labels, g_lp.masked_fill(at, 0.0))):
+            hd, wd = hidden.clone().requires_grad_(True), weight.clone().requires_grad_(True)
+            lp, ent = lm_head_logprobs_and_entropy(hd, wd, lab.to(cuda), temperature, keep_logits_mib=keep_mib)
+            outs, ups = ([lp, ent], [up, g_ent]) if with_entropy else ([lp], [up])
+            grads.append(torch.autograd.grad(outs, [hd, wd], [u.to(cuda) for u in ups]))
+            if not with_entropy:
+                assert (grads[-1][0][at.to(cuda)] == 0).all() and (grads[-1][0][~at.to(cuda)] != 0).any(1).all()
+    for a, b in zip(grads[0] + grads[2], grads[1] + grads[3]):
+        assert torch.equal(a, b)
