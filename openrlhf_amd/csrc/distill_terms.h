@@ -20,7 +20,8 @@ namespace orlhf {
 constexpr int kMaxList = 128;                 // two entries per lane of one wave
 constexpr int64_t kMaxDistillVocab = 520192;  // a bit per element in 64 KiB of LDS, less the static part
 constexpr double kTinyTail = 5.9604644775390625e-08;  // 2^-24
-constexpr double kLogTinyRest = -87.33654475055310898657;  // log 2^-126: the student's tail mass is taken to be at least that
+constexpr double kTinyRest = 1.1754943508222875e-38;       // 2^-126: the student's tail mass is taken to be at least that
+constexpr double kLogTinyRest = -87.33654475055310898657;  // its logarithm
 
 __device__ __forceinline__ double wave_max(double v) {
 #pragma unroll
@@ -235,10 +236,13 @@ __device__ __forceinline__ StudentTerms student_terms(const ListEntries& e, doub
   return r;
 }
 
+// The backward of the unlisted elements goes by r = q / s, the softmax outside the list: its weights are in
+// range however small s is. By q, a student that is sure by more than 75 nats lost the pull of the teacher's
+// tail, t r, to weights below 2^-126.
 struct ListTerms {
-  double loss, other;  // the loss and dL/dz / q of an element that is not listed
+  double loss, other;  // the loss and dL/dz / r of an element that is not listed
   double grad[2];      // dL/dz of this lane's entries (0 where absent)
-  float centre, l2;    // q = 2^((x - centre) cT - l2)
+  float centre, l2;    // r = 2^((x - centre) cT - l2)
 };
 
 // One wave. `sum`: the student's softmax sum without the listed elements. fp64: a few hundred operations of
@@ -260,19 +264,21 @@ __device__ __forceinline__ ListTerms list_terms(const ListEntries& e, const Teac
     lq[i] = ((double)e.x[i] * inv_t - base) - log_total;
     q[i] = e.id[i] >= 0 ? exp(lq[i]) : 0.0;
   }
-  double log_s = some ? (sum.base_t - base) + log(sum.sT) - log_total : -INFINITY;
-  if (log_s < kLogTinyRest) log_s = kLogTinyRest;
+  const double log_rest = log(sum.sT);
+  double log_s = some ? (sum.base_t - base) + log_rest - log_total : -INFINITY;
   const double s = exp(log_s), t = teacher.t;
+  double pull = t;  // t q / s at the least s, in units of r
+  if (log_s < kLogTinyRest) pull = t * exp(log_s - kLogTinyRest), log_s = kLogTinyRest;
   if (kind == ORLHF_DISTILL_REVERSE_TAIL) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) part[i] = e.id[i] >= 0 && q[i] != 0.0 ? q[i] * (lq[i] - e.lp[i]) : 0.0;
-    r.loss = wave_sum(part[0] + part[1]) + (t > 0.0 ? s * (log_s - teacher.log_t) : 0.0);
-    r.other = (log_s - teacher.log_t) - r.loss;
+    r.loss = wave_sum(part[0] + part[1]) + (t > 0.0 ? fmax(s, kTinyRest) * (log_s - teacher.log_t) : 0.0);
+    r.other = s * ((log_s - teacher.log_t) - r.loss);
 #pragma unroll
     for (int i = 0; i < 2; ++i) r.grad[i] = part[i] - q[i] * r.loss;
   } else {
     const double scale = tail ? 1.0 : 1.0 / teacher.mass, all = tail ? teacher.mass + t : 1.0;
-    r.other = all - (t > 0.0 ? t / s : 0.0);
+    r.other = all * s - pull;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const double p = teacher.p[i] * scale;
@@ -281,13 +287,14 @@ __device__ __forceinline__ ListTerms list_terms(const ListEntries& e, const Teac
     }
     r.loss = wave_sum(part[0] + part[1]) + (t > 0.0 ? t * (teacher.log_t - log_s) : 0.0);
   }
-  const double at = base * temperature;
+  const double at = sum.base_t * temperature;
   r.centre = (float)at;
-  r.l2 = (float)((log_total + (at - (double)r.centre) * inv_t) * 1.4426950408889634);
-  if (teacher.n_on == 0) {  // nothing to learn from: no loss, no gradient
-    r.loss = r.other = 0.0;
+  r.l2 = (float)((log_rest + (at - (double)r.centre) * inv_t) * 1.4426950408889634);
+  if (teacher.n_on == 0) r.loss = 0.0;  // nothing to learn from: no loss, no gradient
+  if (teacher.n_on == 0 || !some) {
     r.centre = INFINITY;  // every weight of the backward 0
     r.l2 = 0.0f;
+    r.other = teacher.n_on > 0 && base == -INFINITY ? NAN : 0.0;  // nothing but -inf in the row: no softmax
   }
   if (e.bad) r.loss = NAN;
   return r;

@@ -461,3 +461,43 @@ def test_teacher_logits_of_any_size(cuda, teacher_temperature, shift, scale, n):
             assert abs(l[r].item() - value) <= rel + size, (r, l[r].item(), value)
             w = weight[r].item()
             assert ((gr[r].double().cpu() - w * d).abs() <= w * bound + 1e-37).all(), r
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("rows", [4, 300])
+@pytest.mark.parametrize("vocab", [3001, 70001])
+def test_gradients_of_students_sure_beyond_the_range_of_fp32(cuda, form, dtype, rows, vocab):
+    """The student's mass outside the list is 1e-33 to 1e-37 and each weight there far below the least fp32
+    number, but the teacher's tail still pulls: d / dz = ((P + t) s - t) r with r the softmax outside the list.
+    r is as exact as its sum (d), its stored logarithm (up to 20 in log2 units) and its exponents are."""
+    from openrlhf_amd.models.utils import distill_kl_from_logits, fused_distill_kl_fwd_bwd
+
+    g = torch.Generator().manual_seed(vocab)
+    temperature = 0.25
+    x = torch.randn(rows, vocab, generator=g)
+    listed = torch.stack([torch.randperm(vocab, generator=g)[:3] for _ in range(rows)])
+    gap = (torch.tensor([80.0, 82.5, 84.0, 85.0])[torch.arange(rows) % 4] + math.log(vocab)) * temperature + 0.5 / temperature * 0.9
+    x.scatter_(1, listed, torch.tensor([0.0, -0.5, -1.0]).repeat(rows, 1) + gap.view(-1, 1))
+    x = x.to(TYPES[dtype])
+    lps = torch.log(torch.tensor([[0.6, 0.2, 0.1]])).repeat(rows, 1)
+    weight = (0.5 + torch.rand(rows, generator=g)) * (256.0 if dtype == "fp16" else 1.0)
+    view, idc, lpc = x.cuda(), listed.cuda(), lps.cuda()
+    leaf = view.detach().requires_grad_(True)
+    loss = distill_kl_from_logits(leaf, idc, lpc, temperature, *form)
+    (grad,) = torch.autograd.grad([loss], [leaf], [weight.cuda()])
+    _, grad2 = fused_distill_kl_fwd_bwd(view, idc, lpc, weight.cuda(), temperature, *form, inplace=False)
+    half = torch.finfo(TYPES[dtype]).eps / 2
+    for r, (_, d, x64) in zip(range(4), _reference(view, listed, lps, temperature, form, range(4))):
+        outside = torch.ones(vocab, dtype=torch.bool)
+        outside[listed[r]] = False
+        s = torch.log_softmax(x64 / temperature, -1)[outside].exp().sum().item()
+        assert 2.0 ** -126 < s < 1e-32, s  # what the test is about
+        d = weight[r].item() * d[outside]
+        centred = (x64[outside] - x64[outside].max()).abs() / temperature
+        rel = _sum_error(x64, temperature) + (24 + 4 * centred) * U
+        for gr in (grad, grad2):
+            got = gr[r].double().cpu()[outside]
+            assert ((got - d).abs() <= (half + 2 * rel) * d.abs() + 2 * FLOOR[TYPES[dtype]]).all(), (r, s)
+    if form == ("forward", True):
+        assert (grad[:4].abs().sum(1) > 0.1).all()
