@@ -378,7 +378,7 @@ template <int DT, int MODE>
 __global__ __launch_bounds__(kBlock) void top_logprobs_fwd_kernel(TopArgs a) {
   using E = Elt<DT>;
   __shared__ TopShared sh;
-  extern __shared__ uint64_t shared[];  // block maxima while the row streams by, candidates afterwards
+  extern __shared__ __align__(16) uint64_t shared[];  // block maxima while the row streams by, candidates afterwards
   float* const block_max = (float*)shared;
   const Candidates cand = {shared, sh.n_cand};
   const int tid = threadIdx.x;
@@ -453,7 +453,7 @@ __global__ __launch_bounds__(kBlock) void top_logprobs_fwd_kernel(TopArgs a) {
 template <int MODE>
 __global__ __launch_bounds__(kBlock) void top_logprobs_merge_kernel(TopArgs a) {
   __shared__ TopShared sh;
-  __shared__ uint64_t keys[kCap];
+  __shared__ __align__(16) uint64_t keys[kCap];
   const int64_t row_i = grid_row();
   if (row_i >= a.n_rows || (a.row_mask != nullptr && a.row_mask[row_i] == 0)) return;
   const Candidates cand = {keys, sh.n_cand};

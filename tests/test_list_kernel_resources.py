@@ -1,0 +1,39 @@
+"""What the compiler says about the kernels over a row and a list of tokens (registers, scratch, LDS), on the
+CPU: compiled for gfx950 with the library's own flags, those of the single source included."""
+import functools
+import os
+import re
+import subprocess
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+@functools.lru_cache(maxsize=None)
+def _resources(source):
+    """{mangled kernel name: {"VGPRs": n, "VGPRs Spill": n, "ScratchSize": n, "LDS Size": n}}"""
+    from openrlhf_amd.csrc import build as b
+
+    cmd = [b.find_hipcc(), *b.HIPCC_FLAGS, *b.SOURCE_FLAGS.get(source, []), "-I", os.path.join(ROOT, "include"), "--cuda-device-only",
+           "-c", os.path.join(b.CSRC, source), "-o", os.devnull, "-Rpass-analysis=kernel-resource-usage"]
+    out = subprocess.run(cmd, capture_output=True, text=True)
+    assert out.returncode == 0, out.stderr[-2000:]
+    kernels, name = {}, None
+    for line in out.stderr.splitlines():
+        m = re.search(r"remark:\s+Function Name: (\S+)", line)
+        if m:
+            name = m.group(1)
+            kernels[name] = {}
+            continue
+        m = re.search(r"remark:\s+(VGPRs Spill|VGPRs|ScratchSize|LDS Size)(?: \[[^]]*\])?: (\d+)", line)
+        if m and name:
+            kernels[name][m.group(1)] = int(m.group(2))
+    return kernels
+
+
+def test_candidate_keys_lie_on_16_bytes():
+    """The ranking reads the candidates two keys at a time with 16-byte LDS loads. In the forward kernel they
+    lie in the dynamic LDS, which begins where the static LDS ends."""
+    kernels = {k: v for k, v in _resources("top_logprobs.hip").items() if "top_logprobs_fwd_kernel" in k}
+    assert len(kernels) == 9, sorted(kernels)
+    for k, v in kernels.items():
+        assert v["LDS Size"] > 0 and v["LDS Size"] % 16 == 0, (k, v)
