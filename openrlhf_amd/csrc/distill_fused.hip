@@ -79,6 +79,20 @@ struct ListState {
   int n_on, bad;
 };
 
+// The workgroup's static LDS; the dynamic part holds the two maps and the parked chunks.
+struct OneShared {
+  float lds[kOneWaves][4];
+  float bcast[4];
+  uint32_t ends[2];
+  int keys[2][kSlots];
+  float values[2][kSlots];
+  ListState state[2];
+  uint32_t dirty[2][kOneBlock][2];
+};
+constexpr int64_t kLdsBytes = 160 * 1024;  // of a CU
+static_assert((int64_t)sizeof(OneShared) + 2 * ((kMaxMapped + 127) / 128 * 16) + kParked * kOneBlock * 16 <= kLdsBytes,
+              "the longest row's maps fit");
+
 // Workgroup barrier for what passes through LDS: loads and stores of device memory stay in flight.
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
@@ -98,13 +112,14 @@ template <int DT, int CHUNKS, bool LONG>
 __global__ __launch_bounds__(kOneBlock) void distill_one_pass_kernel(OneArgs a) {
   using E = Elt<DT>;
   constexpr int EPV = E::kPerVec;
-  __shared__ float lds[kOneWaves][4];
-  __shared__ float bcast[4];
-  __shared__ uint32_t ends[2];
-  __shared__ int keys[2][kSlots];
-  __shared__ float values[2][kSlots];
-  __shared__ ListState state[2];
-  __shared__ uint32_t dirty[2][kOneBlock][2];
+  __shared__ OneShared sh;
+  auto& lds = sh.lds;
+  auto& bcast = sh.bcast;
+  auto& ends = sh.ends;
+  auto& keys = sh.keys;
+  auto& values = sh.values;
+  auto& state = sh.state;
+  auto& dirty = sh.dirty;
   extern __shared__ u32x4 maps[];  // two maps, then the parked chunks
   u32x4(*const park)[kOneBlock] = (u32x4(*)[kOneBlock])(maps + a.map_words / 2);
   const uint32_t tid = threadIdx.x, tid16 = tid * 16u, lane = tid % kWave, wave = tid / kWave;
@@ -425,7 +440,6 @@ static int64_t one_pass_max_vocab(int dtype) {
 
 template <int DT, int CHUNKS, bool LONG>
 static int launch_one_pass(const OneArgs& a, unsigned blocks, hipStream_t stream) {
-  static_assert(2 * (kMaxMapped / 8 + 16) + kParked * kOneBlock * 16 + 18432 <= 163840, "LDS of a CU");
   const size_t lds = (size_t)a.map_words * 4 * 2 + (size_t)kParked * kOneBlock * 16;
   // more than the 64 KiB that a launch may ask for by itself
   const hipError_t e = hipFuncSetAttribute((const void*)distill_one_pass_kernel<DT, CHUNKS, LONG>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);

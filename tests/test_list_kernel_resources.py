@@ -37,3 +37,16 @@ def test_candidate_keys_lie_on_16_bytes():
     assert len(kernels) == 9, sorted(kernels)
     for k, v in kernels.items():
         assert v["LDS Size"] > 0 and v["LDS Size"] % 16 == 0, (k, v)
+
+
+def test_one_pass_distillation_fits_the_lds_of_a_cu(lib):
+    """Static LDS as compiled, two maps of the longest row (a bit per element, whole 16-byte words) and the six
+    parked 16-byte chunks of 512 lanes in the 160 KiB of a CU."""
+    from openrlhf_amd import _lib
+
+    longest = max(lib.orlhf_distill_kl_fwd_bwd_max_vocab(t) for t in (_lib.F32, _lib.BF16, _lib.F16))
+    maps, parked = 2 * ((longest + 127) // 128 * 16), 6 * 512 * 16
+    kernels = {k: v for k, v in _resources("distill_fused.hip").items() if "distill_one_pass_kernel" in k}
+    assert len(kernels) == 6, sorted(kernels)
+    for k, v in kernels.items():
+        assert v["LDS Size"] + maps + parked <= 160 * 1024, (k, v)
