@@ -27,7 +27,7 @@ constexpr int kMaxFactor = 4;    // longest row: 4 x the resident part, and two 
 constexpr int64_t kMaxMapped = 376832;
 constexpr int kSlots = 256;      // of the hash table: twice the longest list
 // Chunks of a lane that wait in LDS (its own 16 bytes each, no barrier) from the sum to the gradient: the
-// fp64 arithmetic of the list in between needs their registers (without: 122 registers spilled).
+// fp64 arithmetic of the list in between needs their registers (without: 34 registers of the fp32 body spilled).
 constexpr int kParked = 6;
 
 struct OneArgs {
@@ -147,6 +147,9 @@ __global__ __launch_bounds__(kOneBlock) void distill_one_pass_kernel(OneArgs a) 
   if (tid < 2 * kMaxList) state[tid / kMaxList].id[tid % kMaxList] = -1;
   dirty[0][tid][0] = dirty[0][tid][1] = dirty[1][tid][0] = dirty[1][tid][1] = 0u;
 
+  // Whether this lane's chunk c lies in a row of n vectors; written so that no register per chunk is kept for it.
+  auto within = [&](int c, uint32_t n) { return (int)tid < (int)n - c * kOneBlock; };
+
   u32x4 buf[CHUNKS];
   float xs = -INFINITY;
   int64_t row_i = next_active(blockIdx.x, true);
@@ -233,7 +236,7 @@ __global__ __launch_bounds__(kOneBlock) void distill_one_pass_kernel(OneArgs a) 
     const char* body = row + g.head * E::kSize;
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c)
-      buf[c] = (uint32_t)c * kOneBlock + tid < g.nvec ? load_vec(body + (uint32_t)c * (kOneBlock * 16u) + tid16) : minus_inf_vec<DT>();
+      buf[c] = within(c, g.nvec) ? load_vec(body + (uint32_t)c * (kOneBlock * 16u) + tid16) : minus_inf_vec<DT>();
     if (tid < g.head + g.tail) xs = E::load1(row + (tid < g.head ? tid : g.nvec * EPV + tid) * E::kSize);
   }
   __syncthreads();  // the empty maps and tables
@@ -265,7 +268,7 @@ __global__ __launch_bounds__(kOneBlock) void distill_one_pass_kernel(OneArgs a) 
       for (int c = 0; c < CHUNKS; ++c) {
         float x[EPV];
         E::unpack(pinned(kFromLds && c >= CHUNKS - kParked ? park[c - (CHUNKS - kParked)][tid] : buf[c]), x);
-        if (touched(c)) without.vec(x, (uint32_t)c * kOneBlock + tid);
+        if (touched(c)) without.vec(x, tid, (uint32_t)c * kOneBlock);
 #pragma unroll
         for (int j = 0; j < EPV; ++j) f(x[j], j & 1);
         settle();
@@ -372,17 +375,17 @@ __global__ __launch_bounds__(kOneBlock) void distill_one_pass_kernel(OneArgs a) 
     lds_barrier();
     const float centre = bcast[0], neg_l2 = -bcast[1], coef = bcast[2];
     auto grad_of = [&](float x) { return fast_exp2(fmaf(fmaxf(x - centre, -1.0e30f), cT, neg_l2)) * coef; };
-    auto grad_vec = [&](float (&x)[EPV], uint32_t v, int c) {
+    auto grad_vec = [&](float (&x)[EPV], uint32_t v, uint32_t step, int c) {
 #pragma unroll
       for (int j = 0; j < EPV; ++j) x[j] = grad_of(x[j]);
       if (touched(c)) {
         // one loop over the set bits: unrolled per element the look-ups made half a megabyte of code
-        uint32_t bits = map.vec(v);
+        uint32_t bits = map.vec(v, step);
 #pragma unroll 1
         while (bits != 0u) {
           const int at = __builtin_ctz(bits);
           bits &= bits - 1u;
-          const float value = table.find((int)(g.head + v * EPV + at));
+          const float value = table.find((int)(g.head + (v + step) * EPV + at));
 #pragma unroll
           for (int j = 0; j < EPV; ++j) x[j] = j == at ? value : x[j];
         }
@@ -400,21 +403,20 @@ __global__ __launch_bounds__(kOneBlock) void distill_one_pass_kernel(OneArgs a) 
     char* obody = out_row + g.head * E::kSize;
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c) {
-      const uint32_t v = (uint32_t)c * kOneBlock + tid;
-      if (v < g.nvec) {
+      if (within(c, g.nvec)) {
         float x[EPV];
         E::unpack(pinned(c >= CHUNKS - kParked ? park[c - (CHUNKS - kParked)][tid] : buf[c]), x);
-        grad_vec(x, v, c);
+        grad_vec(x, tid, (uint32_t)c * kOneBlock, c);
         store_vec(obody + (uint32_t)c * (kOneBlock * 16u) + tid16, E::pack(x));
       }
-      buf[c] = v < gn.nvec ? load_vec(nbody + (uint32_t)c * (kOneBlock * 16u) + tid16) : minus_inf_vec<DT>();
+      buf[c] = within(c, gn.nvec) ? load_vec(nbody + (uint32_t)c * (kOneBlock * 16u) + tid16) : minus_inf_vec<DT>();
     }
     if (LONG) {
 #pragma unroll 2
       for (uint32_t v = kResident + tid; v < g.nvec; v += kOneBlock) {
         float x[EPV];
         E::unpack(*(const u32x4*)(tail_body + v * 16u), x);
-        grad_vec(x, v, 63);
+        grad_vec(x, v, 0u, 63);
         store_vec(obody + v * 16u, E::pack(x));
       }
     }

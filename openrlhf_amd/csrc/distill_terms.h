@@ -173,9 +173,11 @@ struct ListMap {
   __device__ __forceinline__ void drop(const RowGeom& g, uint32_t i) const {
     if (i >= g.head && i - g.head < g.nvec * EPV) words[(i - g.head) / 32u] = 0u;
   }
-  __device__ __forceinline__ uint32_t vec(uint32_t v) const {
+  __device__ __forceinline__ uint32_t vec(uint32_t v) const { return vec(v, 0u); }
+  // Of vector v + step, step a known even number: it stays an offset in the instruction.
+  __device__ __forceinline__ uint32_t vec(uint32_t v, uint32_t step) const {
     const uint8_t* b = (const uint8_t*)words;
-    return EPV == 8 ? b[v] : (uint32_t)(b[v >> 1] >> ((v & 1u) * 4u)) & 0xfu;
+    return EPV == 8 ? (b + v)[step] : (uint32_t)((b + (v >> 1))[step >> 1] >> ((v & 1u) * 4u)) & 0xfu;
   }
   __device__ __forceinline__ bool scalar(uint32_t s) const { return (*ends >> s & 1u) != 0u; }
 };
@@ -185,8 +187,8 @@ template <int DT>
 struct WithoutListed {
   ListMap<DT> map;
   template <int N>
-  __device__ __forceinline__ void vec(float (&x)[N], uint32_t v) const {
-    const uint32_t bits = map.vec(v);
+  __device__ __forceinline__ void vec(float (&x)[N], uint32_t v, uint32_t step = 0u) const {
+    const uint32_t bits = map.vec(v, step);
     if (__ballot(bits != 0u) != 0ull) {  // a branch of the wave, hardly ever taken
 #pragma unroll
       for (int j = 0; j < N; ++j) x[j] = (bits >> j & 1u) != 0u ? -INFINITY : x[j];

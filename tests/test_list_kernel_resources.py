@@ -50,3 +50,12 @@ def test_one_pass_distillation_fits_the_lds_of_a_cu(lib):
     assert len(kernels) == 6, sorted(kernels)
     for k, v in kernels.items():
         assert v["LDS Size"] + maps + parked <= 160 * 1024, (k, v)
+
+
+def test_one_pass_distillation_does_not_spill():
+    """A body holds a whole vocabulary row in its registers: nothing else of the kernel may push any of it to
+    scratch memory, in none of the three types, short rows or long."""
+    kernels = {k: v for k, v in _resources("distill_fused.hip").items() if "distill_one_pass_kernel" in k}
+    assert len(kernels) == 6, sorted(kernels)
+    for k, v in kernels.items():
+        assert v["VGPRs Spill"] == 0 and v["ScratchSize"] == 0, (k, v)
