@@ -255,7 +255,7 @@ __global__ __launch_bounds__(kOneBlock) void distill_one_pass_kernel(OneArgs a) 
 
     // chunks of this lane with a listed element (the last bit: any of the streamed ones)
     const uint32_t dirty_lo = dirty[side][tid][0], dirty_hi = dirty[side][tid][1];
-    auto touched = [&](int c) { return __ballot(((c < 32 ? dirty_lo : dirty_hi) >> (c % 32) & 1u) != 0u) != 0ull; };
+    auto mine = [&](int c) { return ((c < 32 ? dirty_lo : dirty_hi) >> (c % 32) & 1u) != 0u; };
     // what of the row the sum sees: all but the listed elements
     auto each = [&](auto&& f, auto&& settle, auto parked) {
       constexpr bool kFromLds = decltype(parked)::value;
@@ -268,7 +268,7 @@ __global__ __launch_bounds__(kOneBlock) void distill_one_pass_kernel(OneArgs a) 
       for (int c = 0; c < CHUNKS; ++c) {
         float x[EPV];
         E::unpack(pinned(kFromLds && c >= CHUNKS - kParked ? park[c - (CHUNKS - kParked)][tid] : buf[c]), x);
-        if (touched(c)) without.vec(x, tid, (uint32_t)c * kOneBlock);
+        if (mine(c)) without.vec(x, tid, (uint32_t)c * kOneBlock);  // never past the row, where the map ends
 #pragma unroll
         for (int j = 0; j < EPV; ++j) f(x[j], j & 1);
         settle();
@@ -295,7 +295,7 @@ __global__ __launch_bounds__(kOneBlock) void distill_one_pass_kernel(OneArgs a) 
     {
       float x[EPV];
       E::unpack(pinned(buf[0]), x);
-      if (touched(0)) without.vec(x, tid);
+      if (mine(0)) without.vec(x, tid);
       ref = x[0];
 #pragma unroll
       for (int j = 1; j < EPV; ++j) ref = fmaxf(ref, x[j]);
@@ -378,7 +378,7 @@ __global__ __launch_bounds__(kOneBlock) void distill_one_pass_kernel(OneArgs a) 
     auto grad_vec = [&](float (&x)[EPV], uint32_t v, uint32_t step, int c) {
 #pragma unroll
       for (int j = 0; j < EPV; ++j) x[j] = grad_of(x[j]);
-      if (touched(c)) {
+      if (mine(c)) {
         // one loop over the set bits: unrolled per element the look-ups made half a megabyte of code
         uint32_t bits = map.vec(v, step);
 #pragma unroll 1

@@ -501,3 +501,27 @@ def test_gradients_of_students_sure_beyond_the_range_of_fp32(cuda, form, dtype, 
             assert ((got - d).abs() <= (half + 2 * rel) * d.abs() + 2 * FLOOR[TYPES[dtype]]).all(), (r, s)
     if form == ("forward", True):
         assert (grad[:4].abs().sum(1) > 0.1).all()
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("vocab,dtype", [(9, "bf16"), (33, "fp32"), (515, "fp16"), (4096, "bf16"), (4103, "fp16"), (2051, "fp32"),
+                                         (151937, "bf16"), (77827, "fp32"), (155651, "fp16")])
+def test_lists_at_the_ends_of_a_row(cuda, form, vocab, dtype):
+    """The first and last tokens listed: the bits next to the map's end, lanes whose chunk the row ends in, and
+    the elements off the 16-byte grid, in one pass and in two launches."""
+    from openrlhf_amd.models.utils import distill_kl_from_logits, fused_distill_kl_fwd_bwd
+
+    view, _, _, g = _case(270, vocab, 4, dtype, vocab, pad=3, offset=1)
+    k = min(vocab, 8)
+    ids = torch.cat([torch.arange((k + 1) // 2), vocab - 1 - torch.arange(k // 2)]).repeat(270, 1)
+    lps = torch.log_softmax(torch.randn(270, k, generator=g), -1) - 0.2
+    scale = 64.0 if dtype == "fp16" else 1.0
+    weight = (0.2 + torch.rand(270, generator=g)) * scale
+    few = [0, 1, 268, 269]
+    leaf = view.detach().requires_grad_(True)
+    loss = distill_kl_from_logits(leaf, ids.cuda(), lps.cuda(), 0.8, *form)
+    (grad,) = torch.autograd.grad([loss], [leaf], [weight.cuda()])
+    _check(view, ids, lps, 0.8, form, loss.detach().cpu(), grad, weight, few)
+    before = view.clone()
+    loss, grad = fused_distill_kl_fwd_bwd(view, ids.cuda(), lps.cuda(), weight.cuda(), 0.8, *form)
+    _check(before, ids, lps, 0.8, form, loss.cpu(), grad, weight, few)
