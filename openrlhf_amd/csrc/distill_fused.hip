@@ -301,9 +301,12 @@ __global__ __launch_bounds__(kOneBlock) void distill_one_pass_kernel(OneArgs a) 
       for (int j = 1; j < EPV; ++j) ref = fmaxf(ref, x[j]);
       ref = wave_max(ref) * cT;
     }
+    // A wave past the end of a short row has nothing to refer to: reference 0 for its sum of nothing. (Another
+    // wave without a finite first chunk gives NaN here, and the row takes the exact sums below.)
+    const bool idle = wave != 0u && wave * kWave >= g.nvec;
     float acc[2] = {0.0f, 0.0f};
     {
-      const float neg = -ref;
+      const float neg = idle ? 0.0f : -ref;
       each([&](float x, int k) { acc[k] += fast_exp2(fmaf(x, cT, neg)); },
            [&] { asm volatile("" : "+v"(acc[0]), "+v"(acc[1])); }, std::false_type{});
     }

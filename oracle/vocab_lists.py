@@ -45,7 +45,7 @@ def distill_kl_row(logits, ids, teacher, temperature=1.0, teacher_temperature=1.
         if i >= 0 and v != -math.inf:
             listed.setdefault(i, []).append(v / teacher_temperature)
     log_q = torch.log_softmax(logits / temperature, dim=-1)
-    zero = logits.sum() * 0.0
+    zero = torch.where(torch.isfinite(logits), logits, 0.0).sum() * 0.0  # masked logits may be -inf
     if not listed:
         return zero
     joined = lambda off: {i: torch.logsumexp(torch.tensor(v, dtype=torch.float64) - off, 0).item() for i, v in listed.items()}  # noqa: E731

@@ -525,3 +525,35 @@ def test_lists_at_the_ends_of_a_row(cuda, form, vocab, dtype):
     before = view.clone()
     loss, grad = fused_distill_kl_fwd_bwd(view, ids.cuda(), lps.cuda(), weight.cuda(), 0.8, *form)
     _check(before, ids, lps, 0.8, form, loss.cpu(), grad, weight, few)
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("vocab,dtype", [(700, "bf16"), (1500, "fp32"), (3584, "fp16"), (3600, "bf16"), (2100, "fp32")])
+def test_short_rows_and_blocked_stretches_in_one_pass(cuda, form, vocab, dtype):
+    """Rows that leave waves of the workgroup idle, next to rows whose first or later stretches are -inf (a
+    wave then has nothing finite to refer to although it has elements that count)."""
+    from openrlhf_amd.models.utils import fused_distill_kl_fwd_bwd
+
+    view, ids, lps, g = _case(256, vocab, 5, dtype, vocab + 2)
+    for r, (lo, hi) in enumerate([(0, vocab // 2), (vocab // 2, vocab), (0, min(512, vocab // 3)), (0, vocab - 3), (0, 0)]):
+        view[r, lo:hi] = -math.inf
+        view[r] -= 20.0 * r  # references that differ from 0
+    ids[:5] = torch.arange(vocab // 4, vocab // 4 + 5)
+    ids[:5, 0] = vocab - 1
+    for r in range(5):
+        view[r, ids[r].cuda()] = torch.randn(5, generator=g).to(view.dtype).cuda() - 20.0 * r
+    lps[:5] = torch.log_softmax(torch.randn(5, 5, generator=g), -1) - 0.3
+    before = view.clone()
+    weight = torch.ones(256) * (64.0 if dtype == "fp16" else 1.0)
+    loss, grad = fused_distill_kl_fwd_bwd(view, ids.cuda(), lps.cuda(), weight.cuda(), 1.0, *form)
+    assert loss.isfinite().all() and grad.isfinite().all()
+    few = range(7)
+    for r, (want, d, x) in zip(few, _reference(before, ids, lps, 1.0, form, few)):
+        lq = torch.log_softmax(x, -1)
+        rel = _sum_error(x, 1.0)
+        ratios = 2.0 if form[0] == "forward" else 4.0 + 2 * lq[lq > -math.inf].abs().max().item()
+        assert abs(loss[r].item() - want) <= ratios * rel + 2 * U * abs(want), (r, loss[r].item(), want)
+        w, d = weight[r].item(), torch.nan_to_num(d)
+        half = torch.finfo(TYPES[dtype]).eps / 2
+        bound = w * (ratios * (d.abs() + lq.exp()) * (2 * rel + 8 * U) + 4 * U)
+        assert ((grad[r].double().cpu() - w * d).abs() <= half * w * d.abs() + bound + FLOOR[TYPES[dtype]]).all(), r
