@@ -457,7 +457,28 @@ def distill_kl_from_logits(
                             inplace_backward, row_mask)
 
 
-_ONE_PASS_ROWS = 256
+_ONE_PASS_ROUND = 256        # rows that a round of the one-pass kernel takes: one per CU
+_ONE_PASS_RESIDENT = 311296  # bytes of a row that stay on a CU; a longer row's rest is streamed twice
+_ONE_PASS_BYTES = 220 << 10
+
+
+def _one_pass_pays(n_rows, row_bytes):
+    """Whether the one-pass kernel is the faster route. A round of it costs a fixed 11 to 15 us beside the row's
+    bytes (the list, the sum with no load in flight) and the last round as much as a full one, while the two
+    launches cost 3 passes over the bytes there are. So rows have to be long and rounds full: bytes of a
+    resident row x share of the rounds' slots that hold one, against 220 KiB. Measured (us, one pass / two
+    launches, k = 64): bf16 8192 x 151936 1172 / 1350, x 128256 1085 / 1166, x 100000 958 / 946, x 65536 833 /
+    597, x 2048 470 / 119; fp32 4096 x 77824 660 / 690, x 64000 603 / 576; bf16 x 151936 257 rows 76 / 62, 384 80 / 82,
+    512 84 / 97, 513 117 / 112, 768 125 / 139. Rows beyond the resident part pay for up to two rounds, where the
+    two launches have few rows to work on (bf16 x 200000: 512 rows 113 / 123, 2048 rows 470 / 456). One whole
+    round is ahead at any length, for its single launch (2048 elements 20 / 31, 151936 elements 42 / 59);
+    fewer rows leave CUs idle, and the two launches cut them."""
+    if n_rows <= _ONE_PASS_ROUND:
+        return n_rows == _ONE_PASS_ROUND
+    rounds = -(-n_rows // _ONE_PASS_ROUND)
+    if row_bytes > _ONE_PASS_RESIDENT and rounds > 2:
+        return False
+    return min(row_bytes, _ONE_PASS_RESIDENT) * n_rows >= _ONE_PASS_BYTES * rounds * _ONE_PASS_ROUND
 
 
 @torch.no_grad()
@@ -475,9 +496,9 @@ def fused_distill_kl_fwd_bwd(
 ) -> Tuple[torch.Tensor, torch.Tensor]:
     """Forward and backward of ``sum(weights * distill_kl_from_logits(...))`` for weights ``[...]`` known
     up front (``mask / n_tokens``). Returns ``(loss [...], d / d logits)``; with ``inplace=True`` the
-    gradient overwrites the logits storage. From 256 positions on every row is read once and written once
-    (2 x V x itemsize bytes instead of 3 x) where it fits on a CU. Not an autograd function: the gradient
-    is returned."""
+    gradient overwrites the logits storage. Batches of long rows (from about 220 KiB on) are read once and
+    written once (2 x V x itemsize bytes instead of 3 x); where that does not pay, the forward and the
+    backward kernel run one after the other. Not an autograd function: the gradient is returned."""
     require_gpu(logits, weights)
     c = _DistillCall(logits, teacher_ids, teacher_log_probs, temperature, kl, tail, teacher_temperature, row_mask)
     if weights.shape != c.batch_shape:
@@ -486,9 +507,7 @@ def fused_distill_kl_fwd_bwd(
     inplace = inplace and c.aliases
     grad_stride = c.row_stride if inplace else c.vocab
     lib = _lib.load()
-    # one workgroup per CU holds a whole row: with fewer rows than a GPU's 256 CUs some would stand idle,
-    # and the two launches cut such rows (8192 x 151936 bf16: one pass 1164 us, two launches 1346 us)
-    one_pass = (c.n_rows >= _ONE_PASS_ROWS and c.vocab <= lib.orlhf_distill_kl_fwd_bwd_max_vocab(c.code)
+    one_pass = (_one_pass_pays(c.n_rows, c.vocab * c.rows.element_size()) and c.vocab <= lib.orlhf_distill_kl_fwd_bwd_max_vocab(c.code)
                 and ((c.row_stride - grad_stride) * c.rows.element_size()) % 16 == 0
                 and (inplace or c.rows.data_ptr() % 16 == 0))
     if not one_pass:

@@ -419,3 +419,17 @@ def test_distill_entries_refuse_bad_arguments(lib):
         _distill_kind("reverse", False)
     with pytest.raises(RuntimeError, match="GPU only"):
         distill_kl_from_logits(torch.zeros(2, 8), torch.zeros(2, 1, dtype=torch.long), torch.zeros(2, 1))
+
+
+def test_one_pass_distillation_rule():
+    """Which batches the one-pass form takes: long rows in full rounds of one row per CU, or one whole round."""
+    from openrlhf_amd.models.utils import _one_pass_pays
+
+    for n in (0, 1, 24, 255):
+        assert not any(_one_pass_pays(n, b) for b in (2, 4096, 303872, 524288))
+    assert all(_one_pass_pays(256, b) for b in (2, 4096, 303872, 524288))
+    for n in (257, 513, 1024, 8192):  # short rows, and one row more than fits a round
+        assert not _one_pass_pays(n, 4096) and not _one_pass_pays(n, 131072)
+    assert not _one_pass_pays(257, 303872) and not _one_pass_pays(257, 607744)
+    assert all(_one_pass_pays(n, 303872) for n in (511, 512, 768, 1024, 8192))
+    assert _one_pass_pays(512, 400000) and not _one_pass_pays(1024, 400000)

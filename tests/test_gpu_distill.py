@@ -557,3 +557,45 @@ def test_short_rows_and_blocked_stretches_in_one_pass(cuda, form, vocab, dtype):
         half = torch.finfo(TYPES[dtype]).eps / 2
         bound = w * (ratios * (d.abs() + lq.exp()) * (2 * rel + 8 * U) + 4 * U)
         assert ((grad[r].double().cpu() - w * d).abs() <= half * w * d.abs() + bound + FLOOR[TYPES[dtype]]).all(), r
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("rows,vocab,k,dtype,temperature,pad,offset,ragged", [
+    (1, 1, 1, "fp32", 1.0, 0, 0, False),
+    (5, 131, 128, "fp16", 1.0, 1, 3, True),
+    (514, 4099, 7, "bf16", 1.0, 0, 0, True),
+    (300, 262144, 100, "fp16", 0.7, 0, 0, True),
+    (530, 50257, 128, "fp32", 1.0, 6, 3, True),
+    (1031, 33, 33, "fp32", 1.3, 3, 1, True),
+    (260, 80001, 11, "fp32", 2.0, 0, 0, False),
+    (257, 376832, 20, "bf16", 1.0, 0, 0, True),
+])
+def test_one_pass_kernel_whatever_the_rule(cuda, monkeypatch, form, rows, vocab, k, dtype, temperature, pad, offset, ragged):
+    """The one-pass kernel (a public C entry) on shapes for which the Python form takes the two launches."""
+    from openrlhf_amd import _lib
+    from openrlhf_amd.models import utils
+
+    used, call = [], utils.call
+    monkeypatch.setattr(utils, "_one_pass_pays", lambda n_rows, row_bytes: True)
+    monkeypatch.setattr(utils, "call", lambda name, *a: (used.append(name), call(name, *a)))
+    assert vocab <= _lib.load().orlhf_distill_kl_fwd_bwd_max_vocab(_lib.dtype_code(torch.empty(0, dtype=TYPES[dtype])))
+    test_loss_and_gradients(cuda, form, rows, vocab, k, dtype, temperature, pad, offset, ragged)
+    assert "orlhf_distill_kl_fwd_bwd" in used  # in place; out of place only rows on the 16-byte grid go through it
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("vocab,dtype", [(33, "fp32"), (515, "fp16"), (4103, "bf16"), (2051, "fp32"), (77827, "fp32")])
+def test_one_pass_kernel_at_the_ends_of_a_row(cuda, monkeypatch, form, vocab, dtype):
+    from openrlhf_amd.models import utils
+
+    monkeypatch.setattr(utils, "_one_pass_pays", lambda n_rows, row_bytes: True)
+    test_lists_at_the_ends_of_a_row(cuda, form, vocab, dtype)
+
+
+@pytest.mark.parametrize("form", FORMS)
+def test_one_pass_kernel_on_rows_that_go_wrong_of_every_type(cuda, monkeypatch, form):
+    from openrlhf_amd.models import utils
+
+    monkeypatch.setattr(utils, "_one_pass_pays", lambda n_rows, row_bytes: True)
+    for vocab, dtype in ((900, "fp32"), (200003, "fp16")):
+        test_one_pass_on_rows_that_go_wrong(cuda, form, vocab, dtype)
