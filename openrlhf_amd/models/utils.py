@@ -452,7 +452,10 @@ def distill_kl_from_logits(
     counts once with the sum of its probabilities; an id past the vocabulary makes the position's loss
     NaN. Positions without an entry, or with ``row_mask`` 0, have loss 0 and no gradient.
     ``inplace_backward=True`` writes the gradient over the logits storage, as in
-    ``logprobs_and_entropy_from_logits``."""
+    ``logprobs_and_entropy_from_logits``. The teacher gets no gradient: ``teacher_log_probs`` that require
+    one are refused."""
+    if teacher_log_probs.requires_grad and torch.is_grad_enabled():
+        raise ValueError("teacher_log_probs requires a gradient and this loss gives it none: pass teacher_log_probs.detach()")
     return _DistillKL.apply(logits, teacher_ids, teacher_log_probs, temperature, kl, tail, teacher_temperature,
                             inplace_backward, row_mask)
 

@@ -433,3 +433,15 @@ def test_one_pass_distillation_rule():
     assert not _one_pass_pays(257, 303872) and not _one_pass_pays(257, 607744)
     assert all(_one_pass_pays(n, 303872) for n in (511, 512, 768, 1024, 8192))
     assert _one_pass_pays(512, 400000) and not _one_pass_pays(1024, 400000)
+
+
+def test_distillation_refuses_a_teacher_that_wants_a_gradient():
+    from openrlhf_amd.models.utils import distill_kl_from_logits
+
+    args = torch.zeros(2, 8), torch.zeros(2, 1, dtype=torch.long), torch.zeros(2, 1, requires_grad=True)
+    with pytest.raises(ValueError, match="detach"):
+        distill_kl_from_logits(*args)
+    with torch.no_grad(), pytest.raises(RuntimeError, match="GPU only"):  # no graph: nothing is lost
+        distill_kl_from_logits(*args)
+    with pytest.raises(RuntimeError, match="GPU only"):
+        distill_kl_from_logits(args[0], args[1], args[2].detach())
