@@ -239,6 +239,13 @@ def _list_workspace(ws_bytes, n_rows, dev):
     return ws, None if torch.cuda.is_current_stream_capturing() else _row_tickets(dev, n_rows)
 
 
+def _refuse_second_derivative(what):
+    """For backwards that are kernels: with ``create_graph=True`` their result would enter the graph as a constant,
+    and a second derivative would lack the operator's part without a word."""
+    if torch.is_grad_enabled():
+        raise RuntimeError(f"{what} can be differentiated once: its backward does not support create_graph=True")
+
+
 class _TopLogprobs(torch.autograd.Function):
     """logits -> (log-prob of label, entropy, log-probs of the k most likely tokens, their ids)."""
 
@@ -285,6 +292,7 @@ class _TopLogprobs(torch.autograd.Function):
         none = (None,) * 7
         if g_logprob is None and g_entropy is None and g_top is None:
             return none
+        _refuse_second_derivative("top_logprobs_from_logits")
         rows, lab, ids, stats, rmask = ctx.saved_tensors
         dev = rows.device
         n_rows, vocab = rows.shape
@@ -325,7 +333,7 @@ def top_logprobs_from_logits(
     returned), ``return_entropy=False`` the entropy; a label of -100 has log-prob 0 and no gradient.
     ``1 <= k <= 128``.
 
-    Differentiable in the three float outputs (the choice of the tokens is taken as given).
+    Differentiable once in the three float outputs (the choice of the tokens is taken as given).
     ``inplace_backward`` and ``row_mask`` as in ``logprobs_and_entropy_from_logits``; a position with
     mask 0 gets ids -1 and zeros."""
     return _TopLogprobs.apply(logits, labels, int(k), temperature, bool(return_entropy), inplace_backward, row_mask)
@@ -417,6 +425,7 @@ class _DistillKL(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, g_loss):
+        _refuse_second_derivative("distill_kl_from_logits")
         rows, rmask, *saved = ctx.saved_tensors
         g = g_loss.to(torch.float32).contiguous()
         grad = _distill_backward(rows, ctx.row_stride, ctx.k, ctx.temperature, g, saved, rmask, ctx.inplace)
@@ -435,7 +444,7 @@ def distill_kl_from_logits(
     row_mask: Optional[torch.Tensor] = None,
 ) -> torch.Tensor:
     """KL divergence per position between a teacher known by its most likely tokens and the student
-    ``q = softmax(logits / temperature)``; fp32, differentiable in the logits.
+    ``q = softmax(logits / temperature)``; fp32, differentiable once in the logits.
 
     ``teacher_ids`` (int64 or int32) and ``teacher_log_probs``, both ``[..., k]`` with ``k <= 128``, are
     what ``top_logprobs_from_logits(teacher_logits, None, k, temperature)`` returns. With p the teacher's

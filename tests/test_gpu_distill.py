@@ -599,3 +599,18 @@ def test_one_pass_kernel_on_rows_that_go_wrong_of_every_type(cuda, monkeypatch, 
     monkeypatch.setattr(utils, "_one_pass_pays", lambda n_rows, row_bytes: True)
     for vocab, dtype in ((900, "fp32"), (200003, "fp16")):
         test_one_pass_on_rows_that_go_wrong(cuda, form, vocab, dtype)
+
+
+def test_second_derivatives_are_refused(cuda):
+    from openrlhf_amd.models.utils import distill_kl_from_logits, top_logprobs_from_logits
+
+    view, ids, lps, _ = _case(3, 50, 4, "fp32", 1)
+    leaf = view.detach().requires_grad_(True)
+    loss = distill_kl_from_logits(leaf, ids.cuda(), lps.cuda())
+    with pytest.raises(RuntimeError, match="differentiated once"):
+        torch.autograd.grad(loss.sum(), [leaf], create_graph=True)
+    assert torch.autograd.grad(loss.sum(), [leaf])[0].isfinite().all()
+    _, entropy, top, _ = top_logprobs_from_logits(leaf, None, 4)
+    with pytest.raises(RuntimeError, match="differentiated once"):
+        torch.autograd.grad(top.sum() + entropy.sum(), [leaf], create_graph=True)
+    assert torch.autograd.grad(top.sum(), [leaf])[0].isfinite().all()
