@@ -23,7 +23,7 @@ GROUP_IDENTITY, GROUP_RLOO, GROUP_BASELINE, GROUP_NORM = 0, 1, 2, 3
 DISTILL_FORWARD_TAIL, DISTILL_FORWARD, DISTILL_REVERSE_TAIL = 0, 1, 2
 PAIR_DPO_SIGMOID, PAIR_DPO_IPO, PAIR_LOGSIGMOID, PAIR_LOGEXP = 0, 1, 2, 3
 
-ABI_VERSION = 23
+ABI_VERSION = 24
 UNPAD_TILE = 2048  # ORLHF_UNPAD_TILE
 LIST_MAX = 128  # longest list of tokens per vocabulary row (alternatives, a teacher's top tokens)
 
@@ -168,6 +168,9 @@ def load(path=None):
             "Run `python -m openrlhf_amd.csrc.build` (needs hipcc); there is no CPU fallback."
         )
     lib = ctypes.CDLL(path)
+    got = lib.orlhf_version() if hasattr(lib, "orlhf_version") else 0  # before the symbols: an older library lacks some
+    if got != ABI_VERSION:
+        raise ImportError(f"{path}: ABI version {got}, binding expects {ABI_VERSION}; rebuild it")
     missing = [name for name in SIGNATURES if not hasattr(lib, name)]
     if missing:
         raise ImportError(f"{path} lacks symbols declared in include/openrlhf_amd.h: {missing}; rebuild it")
@@ -175,9 +178,6 @@ def load(path=None):
         fn = getattr(lib, name)
         fn.restype = restype
         fn.argtypes = argtypes
-    got = lib.orlhf_version()
-    if got != ABI_VERSION:
-        raise ImportError(f"{path}: ABI version {got}, binding expects {ABI_VERSION}")
     _lib = lib
     return lib
 

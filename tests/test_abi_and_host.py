@@ -445,3 +445,24 @@ def test_distillation_refuses_a_teacher_that_wants_a_gradient():
         distill_kl_from_logits(*args)
     with pytest.raises(RuntimeError, match="GPU only"):
         distill_kl_from_logits(args[0], args[1], args[2].detach())
+
+
+def test_an_older_library_is_refused_by_its_version(tmp_path):
+    """A library of an earlier ABI version, which lacks entry points added since, is named by its version."""
+    import shutil
+    import subprocess
+
+    from openrlhf_amd import _lib
+
+    gcc = shutil.which("gcc") or shutil.which("cc")
+    if gcc is None:
+        pytest.skip("no C compiler")
+    for name, source in (("old", "int orlhf_version(void) { return 23; }"), ("none", "int other(void) { return 0; }")):
+        (tmp_path / f"{name}.c").write_text(source)
+        subprocess.run([gcc, "-shared", "-fPIC", "-o", str(tmp_path / f"{name}.so"), str(tmp_path / f"{name}.c")], check=True)
+    before = _lib._lib
+    with pytest.raises(ImportError, match=f"ABI version 23, binding expects {_lib.ABI_VERSION}"):
+        _lib.load(str(tmp_path / "old.so"))
+    with pytest.raises(ImportError, match="ABI version 0"):
+        _lib.load(str(tmp_path / "none.so"))
+    assert _lib._lib is before
