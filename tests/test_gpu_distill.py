@@ -614,3 +614,53 @@ def test_second_derivatives_are_refused(cuda):
     with pytest.raises(RuntimeError, match="differentiated once"):
         torch.autograd.grad(top.sum() + entropy.sum(), [leaf], create_graph=True)
     assert torch.autograd.grad(top.sum(), [leaf])[0].isfinite().all()
+
+
+# The forms above once more through the one-pass kernel, where the rule gives their sizes to the two launches.
+@pytest.fixture
+def one_pass(monkeypatch):
+    from openrlhf_amd.models import utils
+
+    used, call = [], utils.call
+    monkeypatch.setattr(utils, "_one_pass_pays", lambda n_rows, row_bytes: True)
+    monkeypatch.setattr(utils, "call", lambda name, *a: (used.append(name), call(name, *a)))
+    yield
+    assert "orlhf_distill_kl_fwd_bwd" in used
+
+
+@pytest.mark.parametrize("rows", [3, 600])
+def test_one_pass_kernel_on_another_stream_and_in_a_replayed_graph(cuda, one_pass, rows):
+    test_other_stream_and_replayed_graph_give_the_same_bits(cuda, rows)
+
+
+@pytest.mark.parametrize("n", [30, 1200])
+def test_one_pass_kernel_with_masked_rows_and_weights_of_zero(cuda, one_pass, n):
+    test_masked_rows_weights_of_zero_and_teacher_temperature(cuda, n)
+
+
+def test_one_pass_kernel_as_the_operators_are_used(cuda, one_pass):
+    test_teacher_targets_to_aggregated_student_loss(cuda)
+
+
+@pytest.mark.parametrize("form", FORMS)
+def test_one_pass_kernel_keeps_digits_and_range(cuda, one_pass, form):
+    test_small_divergences_keep_their_digits(cuda, form, 33000, "bf16", 530)
+    test_small_divergences_keep_their_digits(cuda, form, 2100, "fp32", 300)
+    for dtype in ("fp32", "bf16", "fp16"):
+        test_gradients_of_students_sure_beyond_the_range_of_fp32(cuda, form, dtype, 300, 70001)
+        test_gradients_of_students_sure_beyond_the_range_of_fp32(cuda, form, dtype, 4, 3001)
+
+
+@pytest.mark.parametrize("teacher_temperature,shift,scale", [(1.0, 1000.0, 3.0), (0.05, 40.0, 3.0), (1.0, -720.0, 2.0), (2.0, 3.0e38, 0.0)])
+def test_one_pass_kernel_with_teacher_logits_of_any_size(cuda, one_pass, teacher_temperature, shift, scale):
+    test_teacher_logits_of_any_size(cuda, teacher_temperature, shift, scale, 300)
+
+
+def test_one_pass_kernel_with_every_row_masked_out(cuda, one_pass):
+    from openrlhf_amd.models.utils import fused_distill_kl_fwd_bwd
+
+    view, ids, lps, _ = _case(700, 2051, 5, "bf16", 6, pad=5)
+    poison = torch.full_like(view, math.nan)
+    loss, grad = fused_distill_kl_fwd_bwd(poison, ids.cuda(), lps.cuda(), torch.ones(700, device="cuda"),
+                                          row_mask=torch.zeros(700, device="cuda"))
+    assert (loss == 0).all() and (grad == 0).all()
