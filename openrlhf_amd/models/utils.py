@@ -448,7 +448,8 @@ def distill_kl_from_logits(
 
     ``teacher_ids`` (int64 or int32) and ``teacher_log_probs``, both ``[..., k]`` with ``k <= 128``, are
     what ``top_logprobs_from_logits(teacher_logits, None, k, temperature)`` returns. With p the teacher's
-    probabilities, t = 1 - sum p and s the student's probability of everything outside the list:
+    probabilities, t = 1 - sum p and s the student's probability of everything outside the list (s at
+    least 2^-126):
 
       * ``kl="forward", tail=True``: ``sum p log(p / q) + t log(t / s)``, the divergence of the two
         distributions over the listed tokens and one outcome for the rest;
